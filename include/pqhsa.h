@@ -446,6 +446,59 @@ int pqhsa_hybrid_attend_paged(const void *q, int32_t q_dtype, void *out,
                               size_t workspace_bytes, void *stream);
 
 /*
+ * Dense attention over the whole cache, and eviction from it by accumulated attention weight.  They
+ * need no index: they serve prompts before there is one, layers or contexts kept dense, and caches
+ * that have to shrink.  No counterpart in the reference.
+ *
+ * The score rule.  Row i of a sequence is the token at position i, key j the one at position j:
+ *   z = scale * <q_i, k_j>;  z = softcap * tanh(z / softcap) if softcap > 0;  z -= slopes[head] * |i - j|
+ * and the row sees key j when j lies in the sequence, docs[b, i] == docs[b, j], and either
+ * j <= i and (window == 0 or i - j < window), or j < the sequence's prefix.  (A prefix with a window
+ * keeps the first tokens in sight, a prefix as long as the sequence lifts the causal order.)  Masked
+ * keys may hold anything, infinities and NaN included.  A row that sees nothing gives 0, its
+ * log-sum-exp -inf.  Positions are slots of the cache: after an eviction distances count the keys
+ * that are left.
+ */
+typedef struct pqhsa_score {
+    float scale;
+    float softcap;           /* 0: none */
+    int32_t window;          /* 0: none */
+    int32_t prefix;          /* of every sequence, when prefixes is NULL */
+    const int32_t *prefixes; /* device [B] or NULL */
+    const float *slopes;     /* device [H * G] or NULL */
+    const int32_t *docs;     /* device [B, docs_stride] or NULL: document of every position */
+    int64_t docs_stride;     /* >= n_max */
+} pqhsa_score;
+
+/* Accumulated attention weight per key: out[b, h, j] = decay * in[b, h, j] + the weights that the rows of
+ * the call (all G heads of the group, the last `rows` rows of each sequence) give key j, for j below the
+ * sequence's length; other entries of out are left as they are.  in: NULL = zeros, or out itself. */
+typedef struct pqhsa_mass {
+    const float *in;    /* device [B, H, stride] */
+    float *out;         /* device [B, H, stride] */
+    int64_t stride;     /* >= n_max */
+    float decay;
+    int32_t rows;       /* prompts: rows per sequence that count; 0 = all */
+} pqhsa_mass;
+
+/*
+ * One new token per sequence over its whole cache: the row at position seq_lens[b] - 1, whose K/V row
+ * is in the cache already.  q, out [B, H * G, 128] of the cache's dtype; strides in elements, rows
+ * 16-byte aligned, G <= 16.  `blocks`: blocks the paged cache holds; a block-table entry outside
+ * [0, blocks) masks its keys (contiguous: ignored).  n_max: a HARD bound of the lengths (a longer
+ * sequence is taken as having n_max tokens) that sizes the launch.  lse f32 [B, H * G], mass: may be
+ * NULL.  workspace: 256-byte aligned, of the bytes the function below names, used during the call only.
+ * The key range is split over workgroups and joined by a second launch where one does not suffice.
+ */
+size_t pqhsa_dense_attend_workspace_bytes(int32_t B, int32_t H, int32_t G, int32_t n_max,
+                                          const pqhsa_score *score, int32_t with_mass);
+int pqhsa_dense_attend_paged(const void *q, int32_t q_dtype, int64_t q_stride_row, int64_t q_stride_head,
+                             void *out, int64_t out_stride_row, int64_t out_stride_head,
+                             const pqhsa_kv_view *kv, int32_t blocks, int32_t B, int32_t H, int32_t G,
+                             const int32_t *seq_lens, int32_t n_max, const pqhsa_score *score, float *lse,
+                             const pqhsa_mass *mass, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * Paged-KV readers (benchmarks/vllm_backend/paged_kv_fa.py:95-156).  Both copy rows of
  * sequence `seq` out of the paged cache into contiguous [H, count, 128] K and V tensors of
  * the cache dtype: a token range [start, start + count), or per-head token positions

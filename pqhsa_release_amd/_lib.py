@@ -67,6 +67,15 @@ class Select(ctypes.Structure):
                 ("n_mean", c_int32)]
 
 
+class Score(ctypes.Structure):
+    _fields_ = [("scale", c_float), ("softcap", c_float), ("window", c_int32), ("prefix", c_int32),
+                ("prefixes", c_void_p), ("slopes", c_void_p), ("docs", c_void_p), ("docs_stride", c_int64)]
+
+
+class Mass(ctypes.Structure):
+    _fields_ = [("in_", c_void_p), ("out", c_void_p), ("stride", c_int64), ("decay", c_float), ("rows", c_int32)]
+
+
 SELECT_GENERAL_PATH = 1
 SELECT_ONE_LAUNCH = 2
 SELECT_SHARE_ROWS = 4
@@ -137,6 +146,10 @@ SIGNATURES = {
                                             c_int32, c_void_p, c_void_p, c_void_p]),
     "pqhsa_block_reduce": (ctypes.c_int, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
     "pqhsa_decode_step_launches": (c_int32, [_P(Index), c_int32, c_int32, _P(Select), c_int32]),
+    "pqhsa_dense_attend_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, _P(Score), c_int32]),
+    "pqhsa_dense_attend_paged": (ctypes.c_int, [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int64, c_int64, _P(KvView),
+                                                c_int32, c_int32, c_int32, c_int32, c_void_p, c_int32, _P(Score), c_void_p,
+                                                _P(Mass), c_void_p, c_size_t, c_void_p]),
     "pqhsa_gather_probe": (ctypes.c_int, [_P(KvView), c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p]),
 }
 

@@ -1,0 +1,155 @@
+// What the dense attention kernels share: the score rule, which keys a row sees, the matrix-core
+// operand types and the partial results of a split key range with their join.
+#pragma once
+
+#include <math.h>
+
+#include "common.h"
+
+namespace pqhsa {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// A running maximum is only moved (and what was summed under it rescaled) when a score passes it by
+// more than this, in log2 units: weights then stay below 2^8, which fp32 sums and 16-bit weights hold
+// without loss, and most tiles need no exchange between lanes at all.
+constexpr float kMaxSlack = 8.0f;
+
+// ---- score rule ---------------------------------------------------------------------
+// Scores are kept in units of log2: z2 = log2(e) * z, so that a weight is one exp2.
+struct ScoreArgs {
+    float scale2;             // scale * log2(e)
+    float in_cap, cap2;       // softcap: z2 = cap2 * tanh(dot * in_cap); in_cap = scale / softcap, cap2 = softcap * log2(e)
+    int capped;
+    int window;               // 0: none
+    int prefix;               // of every sequence when prefixes is NULL
+    const int32_t *prefixes;  // [B]
+    const float *slopes;      // [H * G]
+    const int32_t *docs;      // [B, docs_stride]
+    int64_t docs_stride;
+};
+
+inline ScoreArgs make_score(const pqhsa_score *s) {
+    ScoreArgs a = {};
+    a.scale2 = s->scale * kLog2e;
+    a.capped = s->softcap > 0.0f;
+    if (a.capped) {
+        a.in_cap = s->scale / s->softcap;
+        a.cap2 = s->softcap * kLog2e;
+    }
+    a.window = s->window;
+    a.prefix = s->prefix;
+    a.prefixes = s->prefixes;
+    a.slopes = s->slopes;
+    a.docs = s->docs;
+    a.docs_stride = s->docs_stride;
+    return a;
+}
+
+int validate_score(const pqhsa_score *s, int n_max, const char *what);
+int validate_mass(const pqhsa_mass *m, int n_max, const char *what);
+// host-side bound of the keys a row at the end of a sequence can see
+int64_t visible_bound(const pqhsa_score *s, int64_t n_max);
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// tanh to fp32 accuracy relative to the result: the odd Taylor polynomial to x^13 below 0.45 (next term
+// 0.0015 x^15, under 2e-8 of the result there), (1 - e) / (1 + e) with e = exp(-2 |x|) <= 0.41 above.
+// inf gives 1, NaN stays NaN.
+__device__ inline float tanh_score(float x) {
+    const float y = x * x;
+    float p = 21844.0f / 6081075.0f;
+    p = fmaf(p, y, -1382.0f / 155925.0f);
+    p = fmaf(p, y, 62.0f / 2835.0f);
+    p = fmaf(p, y, -17.0f / 315.0f);
+    p = fmaf(p, y, 2.0f / 15.0f);
+    p = fmaf(p, y, -1.0f / 3.0f);
+    p = fmaf(p * y, x, x);
+    const float e = exp2_fast(-2.0f * kLog2e * fabsf(x));
+    const float big = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
+    return fabsf(x) < 0.45f ? p : copysignf(big, x);
+}
+
+__device__ inline int sequence_length(const int32_t *seq_lens, int b, int n_max) {
+    return min(max(seq_lens[b], 0), n_max);
+}
+__device__ inline int sequence_prefix(const ScoreArgs &s, int b) {
+    return max(s.prefixes ? s.prefixes[b] : s.prefix, 0);
+}
+
+// Byte offset of K/V row (b, h, pos), or -1 where the block table names a block outside the cache (such
+// a key is treated as masked).
+__device__ inline int64_t checked_row_bytes(const KvView &v, int blocks, int b, int h, int pos) {
+    int64_t off;
+    if (v.paged) {
+        const int blk = pos / v.block_size;
+        const int row = pos - blk * v.block_size;
+        const int phys = v.block_table[(int64_t)b * v.max_blocks + blk];
+        if (phys < 0 || phys >= blocks) return -1;
+        off = (int64_t)phys * v.stride_block + (int64_t)row * v.stride_tok + (int64_t)h * v.stride_head;
+    } else {
+        off = (int64_t)b * v.stride_seq + (int64_t)pos * v.stride_tok + (int64_t)h * v.stride_head;
+    }
+    return off * v.esize;
+}
+
+// ---- matrix-core operands of the 2-byte types -----------------------------------------
+template <int DT>
+struct Half16;
+template <>
+struct Half16<PQHSA_BF16> {
+    typedef bf16x8 vec8;
+    static __device__ inline f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+    }
+    static __device__ inline f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+    }
+    // two floats rounded to the type (to nearest even), the first in the low half
+    static __device__ inline uint32_t pack(float lo, float hi) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, bf16x2));
+    }
+    static __device__ inline float low(uint32_t w) { return __uint_as_float(w << 16); }
+    static __device__ inline float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+};
+template <>
+struct Half16<PQHSA_F16> {
+    typedef f16x8 vec8;
+    static __device__ inline f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+    }
+    static __device__ inline f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+    }
+    static __device__ inline uint32_t pack(float lo, float hi) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, f16x2));
+    }
+    static __device__ inline float low(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[0]; }
+    static __device__ inline float high(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[1]; }
+};
+
+// ---- partial results of a split key range, and their join ---------------------------------
+// Row r (query row * heads + head) of split s: part_o[(r * splits + s) * 128 ..] the weighted value sum
+// relative to the maximum m, part_ml[r * splits + s] = (m, l); a split without a visible key has m = -inf,
+// l = 0 and no sums.
+struct JoinArgs {
+    const float *part_o;
+    const float2 *part_ml;
+    int splits;
+    int heads;                 // query heads H * G
+    char *out;
+    int64_t out_row, out_head; // strides in elements
+    float *lse;                // [rows, heads] or NULL
+    const int32_t *row_count;  // rows in use (device), NULL: all
+};
+int launch_join(const JoinArgs &a, int dtype, int64_t rows, hipStream_t stream);
+
+}  // namespace pqhsa

@@ -72,6 +72,8 @@ class KvSource:
     dtype: torch.dtype
     batch: int
     kv_heads: int
+    capacity: int = 0     # tokens a sequence can hold
+    blocks: int = 0       # blocks of a paged cache
 
     def ref(self):
         return ctypes.byref(self.view)
@@ -89,7 +91,7 @@ def kv_contiguous(keys: torch.Tensor, values: torch.Tensor) -> KvSource:
     v.dtype, v.paged = dtype_code(keys.dtype), 0
     v.stride_seq, v.stride_head, v.stride_tok, v.stride_block = keys.stride(0), keys.stride(1), keys.stride(2), 0
     v.block_size, v.max_blocks, v.block_table = 0, 0, None
-    return KvSource(v, (keys, values), keys.dtype, keys.shape[0], keys.shape[1])
+    return KvSource(v, (keys, values), keys.dtype, keys.shape[0], keys.shape[1], keys.shape[2])
 
 
 def kv_paged(kv_cache: torch.Tensor, block_table: torch.Tensor) -> KvSource:
@@ -117,7 +119,8 @@ def kv_paged(kv_cache: torch.Tensor, block_table: torch.Tensor) -> KvSource:
         raise ValueError(f"unsupported FLASH_ATTN kv_cache shape {tuple(kv_cache.shape)}")
     v.dtype, v.paged, v.stride_seq = dtype_code(kv_cache.dtype), 1, 0
     v.max_blocks, v.block_table = block_table.shape[1], block_table.data_ptr()
-    return KvSource(v, (kv_cache, block_table), kv_cache.dtype, block_table.shape[0], heads)
+    return KvSource(v, (kv_cache, block_table), kv_cache.dtype, block_table.shape[0], heads,
+                    block_table.shape[1] * v.block_size, kv_cache.shape[1 if kv_cache.dim() == 5 else 0])
 
 
 # --------------------------------------------------------------------------- device index
@@ -729,6 +732,191 @@ def hybrid_attend_paged(q, out, kv: KvSource, index: DeviceIndex, groups: int, s
                                        float(scale), ws.data_ptr(), ws_bytes, _stream())
     _lib.check(rc, "pqhsa_hybrid_attend_paged")
     return out
+
+
+# --------------------------------------------------------------------------- dense attention
+MAX_GROUPS = 16
+
+
+class ScoreRule:
+    """How a dense attention scores and masks (``pqhsa_score``): ``z = scale <q_i, k_j>``, capped to
+    ``softcap * tanh(z / softcap)``, minus ``slopes[head] * |i - j|``; row i sees key j of its own
+    document (``docs`` int32 ``[B, >= n_max]``, one id per position) if ``j <= i`` and, with a
+    ``window``, ``i - j < window``, or if j lies in the ``prefix`` (an int, or int32 ``[B]``).
+    ``slopes`` is float32 ``[H*G]``.  Positions are slots of the cache."""
+
+    def __init__(self, *, scale: float, softcap: float = 0.0, window: int = 0, prefix: int | torch.Tensor | None = None,
+                 slopes: torch.Tensor | None = None, docs: torch.Tensor | None = None) -> None:
+        s = _lib.Score()
+        s.scale, s.softcap, s.window = float(scale), float(softcap), int(window)
+        if not math.isfinite(s.scale) or not math.isfinite(s.softcap) or s.softcap < 0 or s.window < 0:
+            raise ValueError("scale must be finite, softcap finite and not negative, window not negative")
+        if isinstance(prefix, torch.Tensor):
+            if prefix.dtype != torch.int32 or prefix.ndim != 1 or not prefix.is_contiguous():
+                raise ValueError("prefix must be an int or a contiguous int32 [B] tensor")
+            s.prefixes = prefix.data_ptr()
+        elif prefix is not None:
+            s.prefix = int(prefix)
+            if s.prefix < 0:
+                raise ValueError("prefix must not be negative")
+        if slopes is not None:
+            if slopes.dtype != torch.float32 or slopes.ndim != 1 or not slopes.is_contiguous():
+                raise ValueError("slopes must be a contiguous float32 [H*G] tensor")
+            s.slopes = slopes.data_ptr()
+        if docs is not None:
+            if docs.dtype != torch.int32 or docs.ndim != 2 or docs.stride(1) != 1:
+                raise ValueError("docs must be an int32 [B, positions] tensor with unit stride along the positions")
+            s.docs, s.docs_stride = docs.data_ptr(), docs.stride(0) if docs.shape[0] > 1 else docs.shape[1]
+        self.struct = s
+        self.prefix, self.slopes, self.docs = prefix if isinstance(prefix, torch.Tensor) else None, slopes, docs
+        _need_cuda(*(t for t in (self.prefix, slopes, docs) if t is not None))
+
+    def ref(self):
+        return ctypes.byref(self.struct)
+
+    def check(self, batch: int, heads: int, n_max: int) -> None:
+        if self.prefix is not None and self.prefix.shape[0] != batch:
+            raise ValueError(f"prefix must hold one entry per sequence ({batch})")
+        if self.slopes is not None and self.slopes.shape[0] != heads:
+            raise ValueError(f"slopes must hold one entry per query head ({heads})")
+        if self.docs is not None and (self.docs.shape[0] != batch or self.docs.shape[1] < n_max):
+            raise ValueError(f"docs must be [{batch}, >= {n_max}]")
+
+
+def _one_device(first: torch.Tensor, *others) -> torch.device:
+    """The device all tensors of a call are on."""
+    _need_cuda(first)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device} in one call")
+    return first.device
+
+
+class _on_device:
+    """Makes a tensor's device the current one for a call (nothing to do where it already is)."""
+
+    def __init__(self, device: torch.device) -> None:
+        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def _check_rows(t: torch.Tensor, name: str, heads: int, dtype: torch.dtype) -> None:
+    vec = 16 // t.element_size()
+    if t.ndim != 3 or t.shape[1] != heads or t.shape[2] != HEAD_DIM or t.dtype != dtype:
+        raise ValueError(f"{name} must be [rows, {heads}, {HEAD_DIM}] of the cache's dtype {dtype}, got {tuple(t.shape)} {t.dtype}")
+    if (t.stride(2) != 1 or (t.shape[0] > 1 and t.stride(0) % vec) or (heads > 1 and t.stride(1) % vec)
+            or t.data_ptr() % 16):
+        raise ValueError(f"{name}: last dim contiguous, rows and heads 16-byte aligned")
+
+
+def _row_strides(t: torch.Tensor) -> tuple:
+    return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
+
+
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether two rows of a ``[rows, heads, 128]`` output could share memory (row stride >= heads, or the other way)."""
+    r, h = _row_strides(t)
+    rows, heads = t.shape[0], t.shape[1]
+    if rows <= 1 and heads <= 1:
+        return False
+    if rows <= 1:
+        return h < HEAD_DIM
+    if heads <= 1:
+        return r < HEAD_DIM
+    return not (h >= HEAD_DIM and r >= (heads - 1) * h + HEAD_DIM or r >= HEAD_DIM and h >= (rows - 1) * r + HEAD_DIM)
+
+
+def _check_seq_lens(seq_lens: torch.Tensor, batch: int) -> None:
+    if seq_lens.dtype != torch.int32 or seq_lens.numel() != batch or not seq_lens.is_contiguous():
+        raise ValueError(f"seq_lens must be a contiguous int32 [{batch}] tensor")
+
+
+def _mass_struct(mass, mass_in, decay: float, rows: int, batch: int, heads: int, n_max: int):
+    if mass is None:
+        if mass_in is not None:
+            raise ValueError("mass_in without a mass output")
+        return None
+    for t in (mass, mass_in):
+        if t is not None and (t.dtype != torch.float32 or t.ndim != 3 or tuple(t.shape[:2]) != (batch, heads)
+                              or t.shape[2] < n_max or not t.is_contiguous()):
+            raise ValueError(f"mass must be a contiguous float32 [{batch}, {heads}, >= {n_max}] tensor")
+    if mass_in is not None and mass_in.shape != mass.shape:
+        raise ValueError("mass_in must have the shape of mass")
+    if not math.isfinite(float(decay)) or rows < 0:
+        raise ValueError("decay must be finite, mass_rows not negative")
+    m = _lib.Mass()
+    m.in_, m.out, m.stride = _ptr(mass_in), mass.data_ptr(), mass.shape[2]
+    m.decay, m.rows = float(decay), int(rows)
+    return m
+
+
+def _check_bound(kv: KvSource, n_max: int) -> None:
+    if n_max < 0 or n_max > kv.capacity:
+        raise ValueError(f"n_max {n_max} outside [0, {kv.capacity}], the tokens the cache can hold per sequence")
+
+
+class DenseAttendCall:
+    """Dense attention of one new token per sequence with every argument resolved once: ``run()`` is
+    one C call (``pqhsa_dense_attend_paged``), as for ``DecodeCall``.
+
+    ``q``, ``out`` are ``[B, H*G, 128]`` of the cache's dtype (rows may be strided), ``seq_lens``
+    int32 ``[B]`` counts the cached tokens, the new one included; ``n_max`` bounds them on the host (a
+    longer sequence is taken as having ``n_max`` tokens).  ``lse`` float32 ``[B, H*G]`` receives the
+    log-sum-exp of every row.  ``mass`` float32 ``[B, H, >= n_max]`` receives ``decay * mass_in`` plus
+    the weight the group's rows gave each key (``mass_in``: zeros when absent; may be ``mass``
+    itself).  The call owns its workspace, so calls that may overlap are different objects; a HIP
+    graph that holds ``run()`` keeps using it."""
+
+    def __init__(self, q: torch.Tensor, out: torch.Tensor, kv: KvSource, groups: int, seq_lens: torch.Tensor, *,
+                 n_max: int, rule: ScoreRule, lse: torch.Tensor | None = None, mass: torch.Tensor | None = None,
+                 mass_in: torch.Tensor | None = None, decay: float = 1.0) -> None:
+        b, h, n_max = kv.batch, kv.kv_heads, int(n_max)
+        device = _one_device(q, out, seq_lens, lse, mass, mass_in, *kv.keep, rule.prefix, rule.slopes, rule.docs)
+        if not 1 <= groups <= MAX_GROUPS:
+            raise ValueError(f"groups must be 1 to {MAX_GROUPS}")
+        _check_rows(q, "q", h * groups, kv.dtype)
+        _check_rows(out, "out", h * groups, kv.dtype)
+        if q.shape[0] != b or out.shape[0] != b:
+            raise ValueError(f"q and out must have one row per sequence ({b})")
+        if _overlaps_itself(out):
+            raise ValueError("out: rows overlap in memory")
+        _check_seq_lens(seq_lens, b)
+        _check_bound(kv, n_max)
+        rule.check(b, h * groups, n_max)
+        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (b, h * groups) or not lse.is_contiguous()):
+            raise ValueError(f"lse must be a contiguous float32 [{b}, {h * groups}] tensor")
+        self._mass = _mass_struct(mass, mass_in, decay, 0, b, h, n_max)
+        lib = _lib.load()
+        need = lib.pqhsa_dense_attend_workspace_bytes(b, h, groups, n_max, rule.ref(), int(mass is not None))
+        with _on_device(device):
+            self._ws = torch.empty(need, dtype=torch.uint8, device=device)
+        self._keep = (q, out, kv, seq_lens, rule, lse, mass, mass_in)
+        self.out, self._device, self._fn = out, device, lib.pqhsa_dense_attend_paged
+        self._args = (q.data_ptr(), dtype_code(q.dtype), *_row_strides(q), out.data_ptr(), *_row_strides(out), kv.ref(),
+                      kv.blocks, b, h, groups, seq_lens.data_ptr(), n_max, rule.ref(), _ptr(lse),
+                      None if self._mass is None else ctypes.byref(self._mass), self._ws.data_ptr(), need)
+
+    def run(self, stream: int | None = None) -> torch.Tensor:
+        with _on_device(self._device):
+            rc = self._fn(*self._args, _stream() if stream is None else stream)
+        if rc:
+            _lib.check(rc, "pqhsa_dense_attend_paged")
+        return self.out
+
+
+def dense_attend(q: torch.Tensor, out: torch.Tensor, kv: KvSource, groups: int, seq_lens: torch.Tensor, *, n_max: int,
+                 rule: ScoreRule, lse: torch.Tensor | None = None, mass: torch.Tensor | None = None,
+                 mass_in: torch.Tensor | None = None, decay: float = 1.0) -> torch.Tensor:
+    """One ``DenseAttendCall`` (see there for the arguments), its workspace a temporary of this call."""
+    return DenseAttendCall(q, out, kv, groups, seq_lens, n_max=n_max, rule=rule, lse=lse, mass=mass, mass_in=mass_in,
+                           decay=decay).run()
 
 
 # --------------------------------------------------------------------------- paged readers

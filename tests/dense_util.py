@@ -1,0 +1,192 @@
+"""Seeded problems of the dense attention operators and their evaluation in 64 bits on the CPU, with a
+bound on what a kernel may be off: the inputs are taken as given, so only the roundings inside count."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from pqhsa_release_amd import ops
+
+DIM = 128
+SCALE = 1.0 / math.sqrt(DIM)
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+U = 2.0 ** -24        # half a step of fp32
+
+
+class DenseProblem:
+    """B sequences whose last ``rows[b]`` tokens (possibly more than the sequence has) are query rows.
+
+    ``poison`` fills every place of the cache that no row may look at with NaN and infinities."""
+
+    def __init__(self, lens, rows, *, heads=2, groups=4, dtype=torch.bfloat16, layout="5d", block=16, softcap=0.0,
+                 window=0, prefix=None, slopes=False, docs=0, poison=True, pad=0, seed=0, extra=5, q_gain=1.0):
+        g = torch.Generator().manual_seed(seed)
+        self.lens, self.rows, self.B, self.H, self.G = list(lens), list(rows), len(lens), heads, groups
+        self.dtype, self.n_max = dtype, max([0, *lens])
+        self.softcap, self.window, self.pad = softcap, window, pad
+        self.prefix = prefix
+        self.slopes = torch.rand(heads * groups, generator=g) * 0.05 if slopes else None
+        self.docs = None
+        if docs:
+            self.docs = torch.sort(torch.randint(0, docs, (self.B, self.n_max + 3), generator=g), dim=1).values.to(torch.int32)
+        cap = self.n_max + extra
+        self.K = torch.randn(self.B, heads, cap, DIM, generator=g).mul_(torch.exp(0.3 * torch.randn(DIM, generator=g))).to(dtype)
+        self.V = torch.randn(self.B, heads, cap, DIM, generator=g).to(dtype)
+        total = sum(self.rows)
+        q = 0.5 * torch.randn(total + pad, heads, groups, DIM, generator=g)
+        at = 0
+        for b, r in enumerate(self.rows):
+            for i in range(r):
+                pos = max(self.lens[b] - r + i, 0)
+                pick = torch.randint(0, pos + 1, (heads, groups), generator=g)
+                if self.lens[b]:
+                    q[at + i] += 0.5 * self.K[b, torch.arange(heads)[:, None], pick].float()
+            at += r
+        self.q = (q * q_gain).reshape(total + pad, heads * groups, DIM).to(dtype)
+        self.layout, self.block, self.cap = layout, block, cap
+        self.gen, self.poison = g, poison
+
+    # ---- what a row sees, and the result in 64 bits
+    def visible(self, b):
+        """[rows, len] of sequence b."""
+        n, r = self.lens[b], self.rows[b]
+        i = torch.arange(n - r, n).reshape(-1, 1)
+        j = torch.arange(n).reshape(1, -1)
+        see = j <= i
+        if self.window:
+            see &= i - j < self.window
+        p = self.prefix[b] if isinstance(self.prefix, (list, tuple)) else (self.prefix or 0)
+        see |= j < p
+        if self.docs is not None:
+            d = self.docs[b, :n]
+            see &= d[i.clamp(min=0).reshape(-1)].reshape(-1, 1) == d.reshape(1, -1) if n else see
+        return see & (i >= 0)
+
+    def evaluate(self):
+        """(out, lse, out bound, lse bound, per sequence weights and their relative bound)."""
+        total = sum(self.rows)
+        out = torch.zeros(total, self.H * self.G, DIM, dtype=torch.float64)
+        lse = torch.full((total, self.H * self.G), -math.inf, dtype=torch.float64)
+        tol = torch.zeros_like(out)
+        lse_tol = torch.zeros_like(lse)
+        weights, weight_tol = [], []
+        low = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -22}[self.dtype]
+        at = 0
+        for b in range(self.B):
+            n, r = self.lens[b], self.rows[b]
+            see = self.visible(b)
+            w_b, t_b = torch.zeros(self.H, self.G, r, n, dtype=torch.float64), torch.zeros(self.H, self.G, r, dtype=torch.float64)
+            dist = (torch.arange(n - r, n).reshape(-1, 1) - torch.arange(n).reshape(1, -1)).abs().double()
+            for h in range(self.H):
+                K, V = self.K[b, h, :n].double(), self.V[b, h, :n].double()
+                for g in range(self.G):
+                    hq = h * self.G + g
+                    q = self.q[at : at + r, hq].double()
+                    z = q @ K.T * SCALE
+                    # 128 products summed in fp32 in any order, then scaled: every step half a step off
+                    dz = 132 * U * SCALE * (q.abs() @ K.abs().T)
+                    if self.softcap:
+                        z = self.softcap * torch.tanh(z / self.softcap)   # slope at most 1; tanh itself to 8 half steps
+                        dz = dz + 8 * U * z.abs()
+                    if self.slopes is not None:
+                        bias = float(self.slopes[hq]) * dist
+                        z, dz = z - bias, dz + 3 * U * bias
+                    dz = dz + 3 * U * z.abs()
+                    z = z.masked_fill(~see, -math.inf)
+                    dz = torch.where(see, dz, 0.0).amax(1) if n else torch.zeros(r, dtype=torch.float64)
+                    top = z.amax(1, keepdim=True) if n else torch.full((r, 1), -math.inf, dtype=torch.float64)
+                    alive = (top > -math.inf).reshape(-1)
+                    e = torch.exp(z - torch.where(top > -math.inf, top, torch.zeros_like(top)))
+                    l = e.sum(1)
+                    p = e / torch.where(l > 0, l, torch.ones_like(l)).reshape(-1, 1)
+                    # a weight: the error of its score (and of the maximum's), exp2 to 2 half steps, its sums
+                    rel = 2 * dz + (8 + 2 * 40) * U
+                    a = p @ V.abs()
+                    out[at : at + r, hq] = p @ V
+                    tol[at : at + r, hq] = (HALF_STEP[self.dtype] * 1.001 * (p @ V).abs()
+                                            + a * (2 * rel + n * U / 16 + low + self.weight_rounding()).reshape(-1, 1) + 2.0 ** -25)
+                    lse[at : at + r, hq] = torch.where(alive, top.reshape(-1) + torch.log(l), torch.tensor(-math.inf, dtype=torch.float64))
+                    lse_tol[at : at + r, hq] = dz + (n / 16 + 16) * U + 4 * U * lse[at : at + r, hq].abs().nan_to_num(posinf=0.0)
+                    w_b[h, g], t_b[h, g] = p, 2 * rel + n * U / 16
+            weights.append(w_b)
+            weight_tol.append(t_b)
+            at += r
+        return out, lse, tol, lse_tol, weights, weight_tol
+
+    def weight_rounding(self) -> float:
+        """Relative rounding of the weights that enter the value product (one row per sequence: none
+        beyond the remainder counted above)."""
+        return 0.0
+
+    def mass(self, weights, weight_tol, last=0):
+        """Accumulated weight [B, H, n_max] of the last ``last`` rows (0: all), and its bound."""
+        m = torch.zeros(self.B, self.H, self.n_max, dtype=torch.float64)
+        t = torch.zeros_like(m)
+        for b, (w, rel) in enumerate(zip(weights, weight_tol)):
+            n, r = self.lens[b], self.rows[b]
+            first = max(0, r - last) if last else 0
+            m[b, :, :n] = w[:, :, first:].sum((1, 2))
+            t[b, :, :n] = (w * (rel.unsqueeze(-1) + self.G * (r + 1) * U))[:, :, first:].sum((1, 2)) + 2.0 ** -126
+        return m, t
+
+    # ---- device side
+    def poisoned(self):
+        """K and V as they lie in the cache: places no row sees hold NaN or infinities."""
+        K, V = self.K.clone(), self.V.clone()
+        if self.poison:
+            bad = torch.tensor([math.nan, math.inf, -math.inf]).to(self.dtype)
+            for b in range(self.B):
+                seen = torch.zeros(self.cap, dtype=torch.bool)
+                if self.rows[b] and self.lens[b]:
+                    seen[: self.lens[b]] = self.visible(b).any(0)
+                where = torch.nonzero(~seen).reshape(-1)
+                fill = bad[torch.randint(0, 3, (where.numel(),), generator=self.gen)].reshape(1, -1, 1)
+                K[b, :, where] = fill
+                V[b, :, where] = fill.flip(1)
+        return K, V
+
+    def source(self, device="cuda"):
+        """The cache as the operators take it, pages shuffled; the pages' unused places hold NaN too."""
+        K, V = self.poisoned()
+        if self.layout == "dense":
+            return ops.kv_contiguous(K.to(device), V.to(device))
+        bs = self.block
+        per = -(-self.cap // bs)
+        total = self.B * per + 2
+        order = torch.randperm(total, generator=self.gen)[: self.B * per].reshape(self.B, per)
+        fill = math.nan if self.poison else 0.0
+        if self.layout == "5d":
+            cache = torch.full((2, total, bs, self.H, DIM), fill, dtype=self.dtype)
+            kc, vc = cache[0].transpose(1, 2), cache[1].transpose(1, 2)
+        else:
+            cache = torch.full((total, self.H, bs, 2 * DIM), fill, dtype=self.dtype)
+            kc, vc = cache[..., :DIM], cache[..., DIM:]
+        for b in range(self.B):
+            for j in range(per):
+                c = min(bs, self.cap - j * bs)
+                kc[order[b, j], :, :c] = K[b, :, j * bs : j * bs + c]
+                vc[order[b, j], :, :c] = V[b, :, j * bs : j * bs + c]
+        return ops.kv_paged(cache.to(device), order.to(torch.int32).to(device))
+
+    def rule(self, device="cuda"):
+        prefix = self.prefix
+        if isinstance(prefix, (list, tuple)):
+            prefix = torch.tensor(prefix, dtype=torch.int32, device=device)
+        return ops.ScoreRule(scale=SCALE, softcap=self.softcap, window=self.window, prefix=prefix,
+                             slopes=None if self.slopes is None else self.slopes.to(device),
+                             docs=None if self.docs is None else self.docs.to(device))
+
+    def seq_lens(self, device="cuda"):
+        return torch.tensor(self.lens, dtype=torch.int32, device=device)
+
+
+def check_close(got, want, tol, what):
+    """Every element within its own bound, infinities equal."""
+    got, want = got.double().cpu(), want.double()
+    same = got == want
+    off = torch.where(same, torch.zeros_like(want), (got - want).abs())
+    bad = ~(off <= tol)
+    assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} outside, worst {float((off / tol.clamp(min=1e-300))[bad].nan_to_num(1e9).max()):.3g} "
+                           f"times the bound, first at {torch.nonzero(bad)[0].tolist()}: {got[bad][0]} for {want[bad][0]}")

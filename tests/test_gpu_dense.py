@@ -1,0 +1,231 @@
+"""Dense attention of one new token per sequence (``ops.dense_attend``) against an evaluation in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from pqhsa_release_amd import _lib, ops
+from tests.dense_util import DIM, SCALE, DenseProblem, check_close
+
+gpu = pytest.mark.gpu
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+def run(p, *, mass=False, decay=0.9, strided=False):
+    kv, rule = p.source(), p.rule()
+    B, heads = p.B, p.H * p.G
+    if strided:     # rows inside a wider projection, output rows inside a wider buffer
+        wide = torch.full((B, 3 * heads, DIM), math.nan, dtype=p.dtype, device="cuda")
+        q = wide[:, heads : 2 * heads]
+        q.copy_(p.q.cuda())
+        out = torch.full((B, heads + 1, DIM), 7.0, dtype=p.dtype, device="cuda")[:, :heads]
+    else:
+        q, out = p.q.cuda(), torch.full((B, heads, DIM), math.nan, dtype=p.dtype, device="cuda")
+    lse = torch.full((B, heads), math.nan, device="cuda")
+    m = m_in = None
+    if mass:
+        m_in = torch.rand(B, p.H, p.n_max + 2, generator=torch.Generator().manual_seed(5)).cuda()
+        m = torch.full_like(m_in, 7.0)
+    ops.dense_attend(q, out, kv, p.G, p.seq_lens(), n_max=p.n_max, rule=rule, lse=lse, mass=m, mass_in=m_in, decay=decay)
+    torch.cuda.synchronize()
+    return out, lse, m, m_in
+
+
+def check(p, *, mass=False, strided=False):
+    out, lse, m, m_in = run(p, mass=mass, strided=strided)
+    want, want_lse, tol, lse_tol, weights, weight_tol = p.evaluate()
+    check_close(out, want, tol, "out")
+    check_close(lse, want_lse, lse_tol, "lse")
+    if strided:
+        assert bool((out.as_strided((p.B, DIM), ((p.H * p.G + 1) * DIM, 1), p.H * p.G * DIM) == 7.0).all())
+    if mass:
+        add, t = p.mass(weights, weight_tol)
+        for b, n in enumerate(p.lens):
+            old = m_in[b, :, :n].double().cpu()
+            # in fp32: the decay (0.9 is no fp32 number) and its product each half a step off, then G sums of at
+            # most old + add, each half a step off: (2 + G) 2^-24 of old + add
+            check_close(m[b, :, :n], 0.9 * old + add[b, :, :n], t[b, :, :n] + (2 + p.G) * 2.0 ** -24 * (old + add[b, :, :n]), "mass")
+            assert bool((m[b, :, n:] == 7.0).all()), "entries behind the sequence were written"
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("layout,block", [("5d", 16), ("4d", 16), ("dense", 0), ("5d", 7), ("4d", 1), ("5d", 256)])
+def test_layouts_types_and_ragged_lengths(dtype, layout, block):
+    check(DenseProblem([300, 1, 129, 0, 64], [1] * 5, dtype=dtype, layout=layout, block=block, seed=3), mass=True)
+
+
+@gpu
+@pytest.mark.parametrize("heads,groups", [(1, 1), (1, 16), (3, 7), (8, 4), (2, 5)])
+def test_head_layouts(heads, groups):
+    check(DenseProblem([517, 33], [1, 1], heads=heads, groups=groups, seed=11), mass=True, strided=True)
+
+
+@gpu
+@pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 31, 32, 127, 128, 129, 255, 257, 1000, 5003])
+def test_one_sequence_of_every_tail(length):
+    check(DenseProblem([length], [1], heads=1, groups=3, seed=length, extra=0))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("kw", [dict(softcap=3.0), dict(softcap=50.0, slopes=True), dict(slopes=True), dict(window=1),
+                                dict(window=100), dict(window=100, prefix=4), dict(window=64, prefix=[0, 500, 3, 9]),
+                                dict(docs=4), dict(docs=3, window=90, prefix=30, softcap=10.0, slopes=True),
+                                dict(window=10000), dict(prefix=10000)])
+def test_score_rules(dtype, kw):
+    check(DenseProblem([700, 333, 2, 0], [1] * 4, dtype=dtype, seed=21, **kw), mass=True)
+
+
+@gpu
+def test_long_split_range_and_large_scores():
+    check(DenseProblem([40000, 17], [1, 1], heads=1, groups=2, dtype=HF, seed=5, q_gain=6.0), mass=True)
+
+
+@gpu
+def test_prefilled_lengths_beyond_the_bound_are_cut_to_it():
+    p = DenseProblem([200], [1], heads=1, groups=2, seed=8)
+    out, lse, _, _ = run(p)
+    kv, rule = p.source(), p.rule()
+    longer = torch.tensor([500], dtype=torch.int32, device="cuda")
+    again = torch.empty_like(out)
+    ops.dense_attend(p.q.cuda(), again, kv, 2, longer, n_max=200, rule=rule)
+    assert torch.equal(again, out)
+
+
+@gpu
+def test_block_table_entries_outside_the_cache_mask_their_keys():
+    p = DenseProblem([160], [1], heads=2, groups=2, block=16, poison=False, seed=9)
+    kv = p.source()
+    cache, table = kv.keep
+    table[0, 2], table[0, 5] = -1, kv.blocks
+    out = torch.empty(1, 4, DIM, dtype=p.dtype, device="cuda")
+    ops.dense_attend(p.q.cuda(), out, kv, 2, p.seq_lens(), n_max=160, rule=p.rule())
+    gone = torch.zeros(160, dtype=torch.bool)
+    gone[32:48] = gone[80:96] = True
+    q = DenseProblem([160], [1], heads=2, groups=2, block=16, poison=False, seed=9)
+    q.visible = lambda b: (~gone).reshape(1, -1)
+    want, _, tol, _, _, _ = q.evaluate()
+    check_close(out, want, tol, "out")
+
+
+@gpu
+def test_mass_in_place_over_steps_and_a_replayed_graph():
+    p = DenseProblem([900, 250], [1, 1], heads=2, groups=4, seed=31)
+    kv, rule, q, sl = p.source(), p.rule(), p.q.cuda(), p.seq_lens()
+    out = torch.empty_like(q)
+    mass = torch.zeros(2, 2, 900, device="cuda")
+    call = ops.DenseAttendCall(q, out, kv, 4, sl, n_max=900, rule=rule, mass=mass, mass_in=mass, decay=0.5)
+    seen = []
+    for _ in range(3):
+        call.run()
+        seen.append(mass.clone())
+    eager = out.clone()
+    mass.zero_()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call.run()
+    mass.zero_()
+    for k in range(3):
+        out.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and torch.equal(mass, seen[k]), k
+        ops.dense_attend(q, torch.empty_like(q), kv, 4, sl, n_max=900, rule=rule)   # eager work in between
+
+
+@gpu
+def test_two_streams_with_a_call_each():
+    p = DenseProblem([3001], [1], heads=4, groups=4, seed=41)
+    kv, rule, q, sl = p.source(), p.rule(), p.q.cuda(), p.seq_lens()
+    want = ops.dense_attend(q, torch.empty_like(q), kv, 4, sl, n_max=3001, rule=rule).clone()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.empty_like(q) for _ in streams]
+    calls = [ops.DenseAttendCall(q, o, kv, 4, sl, n_max=3001, rule=rule) for o in outs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, c in zip(streams, calls):
+            with torch.cuda.stream(s):
+                c.run()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+@gpu
+def test_visible_nan_and_infinite_scores_reach_the_output_of_their_row_only():
+    p = DenseProblem([100, 100], [1, 1], heads=1, groups=2, poison=False, seed=51)
+    p.q[0, 1, 5] = math.nan
+    out, lse, _, _ = run(p)
+    assert bool(out[0, 1].isnan().all()) and bool(lse[0, 1].isnan())
+    rest = torch.cat([out[0, :1], out[1]])
+    assert bool(rest.isfinite().all())
+
+
+@gpu
+def test_refusals():
+    p = DenseProblem([64, 30], [1, 1], heads=2, groups=2, seed=1)
+    kv, rule, q, sl = p.source(), p.rule(), p.q.cuda(), p.seq_lens()
+    out = torch.empty_like(q)
+
+    def refused(match=None, q=q, out=out, kv=kv, groups=2, sl=sl, **kw):
+        kw = {"n_max": 64, "rule": rule, **kw}
+        with pytest.raises(ValueError, match=match):
+            ops.dense_attend(q, out, kv, groups, sl, **kw)
+
+    refused("device", q=q.cpu())
+    refused("dtype", q=q.float())
+    refused("q must", groups=1)
+    refused("groups", groups=17)
+    refused("n_max", n_max=kv.capacity + 1)
+    refused("n_max", n_max=-1)
+    refused("seq_lens", sl=sl.long())
+    refused("overlap", out=out[:, :1].expand(-1, 4, -1))
+    refused("aligned", q=torch.empty(2 * 4 * DIM + 1, dtype=p.dtype, device="cuda")[1:].view(2, 4, DIM))
+    refused("mass", mass=torch.zeros(2, 2, 63, device="cuda"))
+    refused("mass", mass=torch.zeros(2, 2, 64, device="cuda", dtype=torch.float64))
+    refused("mass output", mass_in=torch.zeros(2, 2, 64, device="cuda"))
+    refused("decay", mass=torch.zeros(2, 2, 64, device="cuda"), decay=math.inf)
+    refused("lse", lse=torch.zeros(2, 3, device="cuda"))
+    refused("prefix", rule=ops.ScoreRule(scale=SCALE, prefix=torch.zeros(3, dtype=torch.int32, device="cuda")))
+    refused("slopes", rule=ops.ScoreRule(scale=SCALE, slopes=torch.zeros(3, device="cuda")))
+    refused("docs", rule=ops.ScoreRule(scale=SCALE, docs=torch.zeros(2, 63, dtype=torch.int32, device="cuda")))
+
+
+def test_rule_refusals_without_a_gpu():
+    for kw in (dict(scale=math.nan), dict(scale=1.0, softcap=-1.0), dict(scale=1.0, softcap=math.inf), dict(scale=1.0, window=-1),
+               dict(scale=1.0, prefix=-2), dict(scale=1.0, prefix=torch.zeros(2)), dict(scale=1.0, slopes=torch.zeros(2)),
+               dict(scale=1.0, docs=torch.zeros(2, 2))):
+        with pytest.raises(ValueError):
+            ops.ScoreRule(**kw)
+
+
+def test_c_entry_refuses_bad_arguments_before_any_gpu_work():
+    import ctypes
+
+    lib = _lib.load()
+    view, score, mass = _lib.KvView(), _lib.Score(), _lib.Mass()
+    view.k_base = view.v_base = 1 << 20
+    view.dtype, view.stride_tok, view.stride_head, view.stride_seq = _lib.BF16, 128, 1280, 12800
+    score.scale = 1.0
+
+    def call(q=1 << 20, dtype=_lib.BF16, stride=128, B=1, H=1, G=1, n_max=10, mass=None, ws=1 << 20, ws_bytes=1 << 20):
+        return lib.pqhsa_dense_attend_paged(q, dtype, 0, stride, 1 << 20, 0, 128, ctypes.byref(view), 0, B, H, G, 1 << 20, n_max,
+                                            ctypes.byref(score), None, mass, ws, ws_bytes, None)
+
+    assert call(G=17) == -1 and b"16" in lib.pqhsa_last_error()
+    assert call(q=None) == -1 and call(q=(1 << 20) + 8) == -1 and call(stride=4) == -1
+    assert call(dtype=_lib.F32) == -1 and b"dtype" in lib.pqhsa_last_error()
+    assert call(n_max=-1) == -1 and call(ws=(1 << 20) + 16) == -1
+    assert call(n_max=1 << 20, ws_bytes=16) == -3 and b"workspace" in lib.pqhsa_last_error()
+    mass.decay = 1.0
+    assert call(mass=ctypes.byref(mass)) == -1
+    mass.out, mass.stride = 1 << 20, 9
+    assert call(mass=ctypes.byref(mass)) == -1
+    view.paged, view.block_table, view.block_size, view.max_blocks, view.stride_block = 1, 1 << 20, 16, 1, 2048
+    assert call() == -1                      # a paged cache without blocks
+    assert call(B=0) == 0
+    score.scale = math.nan
+    assert call() == -1
