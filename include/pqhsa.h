@@ -499,6 +499,25 @@ int pqhsa_dense_attend_paged(const void *q, int32_t q_dtype, int64_t q_stride_ro
                              const pqhsa_mass *mass, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
+ * Prompt rows over the cache: T packed rows of B sequences, rows cu_rows[b] .. cu_rows[b + 1] (device
+ * i32 [B + 1], ascending from 0) are the LAST tokens of sequence b, whose K/V rows are in the cache
+ * already; a whole prompt has as many rows as its sequence tokens.  q, out [T, H * G, 128] of the
+ * cache's dtype; rows of out and lse past cu_rows[B] are left as they are.  A row in front of its
+ * sequence (more rows than tokens) sees nothing.  lse f32 [T, H * G], mass: may be NULL.  rows_hint:
+ * the largest number of rows of a sequence, 0 = unknown (sizes the launch, results do not depend on
+ * it beyond summation order).  n_max, blocks, workspace: as above; `with_lse` is 0 when lse is NULL.
+ * B * H <= 65535, T * H * G < 2^31, at most 65535 * 128 packed rows (T * G).
+ */
+size_t pqhsa_prompt_attend_workspace_bytes(int64_t T, int32_t B, int32_t H, int32_t G, int32_t n_max,
+                                           int32_t rows_hint, int32_t dtype, int32_t with_lse);
+int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t q_stride_row, int64_t q_stride_head,
+                              void *out, int64_t out_stride_row, int64_t out_stride_head, int64_t T,
+                              const int32_t *cu_rows, const pqhsa_kv_view *kv, int32_t blocks, int32_t B,
+                              int32_t H, int32_t G, const int32_t *seq_lens, int32_t n_max, int32_t rows_hint,
+                              const pqhsa_score *score, float *lse, const pqhsa_mass *mass, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
+/*
  * Paged-KV readers (benchmarks/vllm_backend/paged_kv_fa.py:95-156).  Both copy rows of
  * sequence `seq` out of the paged cache into contiguous [H, count, 128] K and V tensors of
  * the cache dtype: a token range [start, start + count), or per-head token positions

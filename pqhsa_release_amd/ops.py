@@ -919,6 +919,45 @@ def dense_attend(q: torch.Tensor, out: torch.Tensor, kv: KvSource, groups: int, 
                            decay=decay).run()
 
 
+def prompt_attend(q: torch.Tensor, out: torch.Tensor, kv: KvSource, groups: int, cu_rows: torch.Tensor,
+                  seq_lens: torch.Tensor, *, n_max: int, rule: ScoreRule, rows_max: int = 0,
+                  lse: torch.Tensor | None = None, mass: torch.Tensor | None = None, mass_in: torch.Tensor | None = None,
+                  decay: float = 1.0, mass_rows: int = 0) -> torch.Tensor:
+    """Dense attention of packed prompt rows (``pqhsa_prompt_attend_paged``): rows ``cu_rows[b]`` to
+    ``cu_rows[b + 1]`` of ``q``, ``out`` ``[T, H*G, 128]`` are the last tokens of sequence b, whose K/V
+    rows are in the cache already.  Rows past ``cu_rows[B]`` are left as they are.  ``rows_max``, the
+    largest number of rows of a sequence, is a hint that sizes the launch.  ``mass`` receives ``decay *
+    mass_in`` plus the weight that the last ``mass_rows`` rows of every sequence (0: all) gave each key.
+    The other arguments are ``DenseAttendCall``'s; the workspace is a temporary of this call."""
+    b, h, n_max, t = kv.batch, kv.kv_heads, int(n_max), q.shape[0]
+    device = _one_device(q, out, cu_rows, seq_lens, lse, mass, mass_in, *kv.keep, rule.prefix, rule.slopes, rule.docs)
+    if not 1 <= groups <= MAX_GROUPS:
+        raise ValueError(f"groups must be 1 to {MAX_GROUPS}")
+    _check_rows(q, "q", h * groups, kv.dtype)
+    _check_rows(out, "out", h * groups, kv.dtype)
+    if out.shape[0] != t or _overlaps_itself(out):
+        raise ValueError("out must have q's rows, none of which overlap in memory")
+    if cu_rows.dtype != torch.int32 or tuple(cu_rows.shape) != (b + 1,) or not cu_rows.is_contiguous():
+        raise ValueError(f"cu_rows must be a contiguous int32 [{b + 1}] tensor")
+    _check_seq_lens(seq_lens, b)
+    _check_bound(kv, n_max)
+    rule.check(b, h * groups, n_max)
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (t, h * groups) or not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous float32 [{t}, {h * groups}] tensor")
+    m = _mass_struct(mass, mass_in, decay, int(mass_rows), b, h, n_max)
+    lib = _lib.load()
+    rows_max = max(0, min(int(rows_max), t))
+    need = lib.pqhsa_prompt_attend_workspace_bytes(t, b, h, groups, n_max, rows_max, dtype_code(kv.dtype), int(lse is not None))
+    with _on_device(device):
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        rc = lib.pqhsa_prompt_attend_paged(q.data_ptr(), dtype_code(q.dtype), *_row_strides(q), out.data_ptr(),
+                                           *_row_strides(out), t, cu_rows.data_ptr(), kv.ref(), kv.blocks, b, h, groups,
+                                           seq_lens.data_ptr(), n_max, rows_max, rule.ref(), _ptr(lse),
+                                           None if m is None else ctypes.byref(m), ws.data_ptr(), need, _stream())
+    _lib.check(rc, "pqhsa_prompt_attend_paged")
+    return out
+
+
 # --------------------------------------------------------------------------- paged readers
 def paged_gather_range(kv: KvSource, seq: int, start: int, end: int):
     """Token range [start, end) of sequence ``seq`` -> K, V ``[H, n, 128]``."""
