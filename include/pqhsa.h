@@ -518,6 +518,25 @@ int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t q_stride_r
                               size_t workspace_bytes, void *stream);
 
 /*
+ * Eviction: of every stream (b, h) whose sequence has more than `keep` tokens, the first `sink` and the
+ * last `recent` keys and the keys of largest mass among the others are kept, `keep` in all (equal
+ * masses: the lowest positions; ordered by bit pattern as pqhsa_topk_radix orders); shorter sequences
+ * keep everything.  The kept keys' K/V rows are copied in ascending order of position to slots 0, 1, ... of
+ * `dst`, a view of the same B, H and dtype over memory apart from the rows read (another cache, or
+ * other blocks of the same one; the caller frees the old blocks).  Outputs: kept i32 [B, H, keep] old
+ * positions (-1 behind the last), new_lens i32 [B] = min(length, keep), and, unless NULL, mass_out f32
+ * [B, H, mass_out_stride]: the kept keys' masses, zeros behind them (tokens appended later start from
+ * zero).  mass f32 [B, H, mass_stride], mass_out apart from it.  n_max: a HARD bound of the lengths.
+ * keep >= sink + recent; blocks as above: a row of a block outside the old cache is copied as zeros, one
+ * that would go to a block outside the new one is left out.  An index of the old cache does not describe
+ * the new one: it has to be encoded again.
+ */
+int pqhsa_evict(const pqhsa_kv_view *src, int32_t src_blocks, const pqhsa_kv_view *dst, int32_t dst_blocks,
+                int32_t B, int32_t H, const float *mass, int64_t mass_stride, const int32_t *seq_lens,
+                int32_t n_max, int32_t keep, int32_t sink, int32_t recent, int32_t *kept, int32_t *new_lens,
+                float *mass_out, int64_t mass_out_stride, void *stream);
+
+/*
  * Paged-KV readers (benchmarks/vllm_backend/paged_kv_fa.py:95-156).  Both copy rows of
  * sequence `seq` out of the paged cache into contiguous [H, count, 128] K and V tensors of
  * the cache dtype: a token range [start, start + count), or per-head token positions

@@ -12,7 +12,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libpqhsa.so")
 SOURCES = ["api.hip", "lut_build.hip", "scan_select.hip", "scan_emit.hip", "scan_stats.hip", "attend.hip", "encode.hip", "encode_prefilter.hip", "nearest.hip", "decode.hip", "probe.hip", "fused.hip",
-           "dense_attend.hip", "prompt_attend.hip"]
+           "dense_attend.hip", "prompt_attend.hip", "evict.hip"]
 
 FLAGS = [
     "--offload-arch=gfx950",

@@ -958,6 +958,48 @@ def prompt_attend(q: torch.Tensor, out: torch.Tensor, kv: KvSource, groups: int,
     return out
 
 
+def evict(kv: KvSource, dst: KvSource, mass: torch.Tensor, seq_lens: torch.Tensor, *, keep: int, sink: int, recent: int,
+          n_max: int, mass_out: torch.Tensor | None = None):
+    """Keep ``keep`` keys of every sequence and KV head and copy their K/V rows, in ascending order of
+    position, to the first slots of ``dst`` (``pqhsa_evict``): the first ``sink``, the last ``recent``,
+    and of the others those with the largest accumulated weight ``mass`` float32 ``[B, H, >= n_max]``
+    (equal ones: the lowest positions).  Shorter sequences keep everything.  ``dst`` is another cache,
+    or other blocks of the same one (its table names none of the blocks being read; the caller frees
+    those afterwards).  Returns ``(kept, new_lens)``: int32 ``[B, H, keep]`` old positions, -1 behind the
+    last, and int32 ``[B]``.  ``mass_out`` float32 ``[B, H, >= min(keep, n_max)]`` receives the kept keys'
+    weights, zeros behind them.  An index of the old cache does not describe the new one."""
+    b, h, n_max, keep = kv.batch, kv.kv_heads, int(n_max), int(keep)
+    device = _one_device(mass, seq_lens, mass_out, *kv.keep, *dst.keep)
+    if dst.batch != b or dst.kv_heads != h or dst.dtype != kv.dtype:
+        raise ValueError("dst must have the batch, KV heads and dtype of kv")
+    if sink < 0 or recent < 0 or keep < 1 or sink + recent > keep:
+        raise ValueError(f"keep {keep} must be positive and hold sink {sink} + recent {recent}")
+    _check_bound(kv, n_max)
+    left = min(keep, n_max)
+    if dst.capacity < left:
+        raise ValueError(f"dst holds {dst.capacity} tokens per sequence, {left} may be kept")
+    shared = {t.untyped_storage().data_ptr() for t in kv.keep} & {t.untyped_storage().data_ptr() for t in dst.keep}
+    if shared and not (kv.view.paged and dst.view.paged and kv.view.block_table != dst.view.block_table):
+        raise ValueError("dst has to lie apart from kv: another cache, or a block table of its own")
+    _check_seq_lens(seq_lens, b)
+    if mass.dtype != torch.float32 or mass.ndim != 3 or tuple(mass.shape[:2]) != (b, h) or mass.shape[2] < n_max or not mass.is_contiguous():
+        raise ValueError(f"mass must be a contiguous float32 [{b}, {h}, >= {n_max}] tensor")
+    if mass_out is not None and (mass_out.dtype != torch.float32 or mass_out.ndim != 3 or tuple(mass_out.shape[:2]) != (b, h)
+                                 or mass_out.shape[2] < left or not mass_out.is_contiguous()):
+        raise ValueError(f"mass_out must be a contiguous float32 [{b}, {h}, >= {left}] tensor")
+    if mass_out is not None and mass_out.untyped_storage().data_ptr() == mass.untyped_storage().data_ptr():
+        raise ValueError("mass_out must not share memory with mass")
+    lib = _lib.load()
+    with _on_device(device):
+        kept = torch.empty(b, h, keep, dtype=torch.int32, device=device)
+        new_lens = torch.empty(b, dtype=torch.int32, device=device)
+        rc = lib.pqhsa_evict(kv.ref(), kv.blocks, dst.ref(), dst.blocks, b, h, mass.data_ptr(), mass.shape[2],
+                             seq_lens.data_ptr(), n_max, keep, int(sink), int(recent), kept.data_ptr(), new_lens.data_ptr(),
+                             _ptr(mass_out), 0 if mass_out is None else mass_out.shape[2], _stream())
+    _lib.check(rc, "pqhsa_evict")
+    return kept, new_lens
+
+
 # --------------------------------------------------------------------------- paged readers
 def paged_gather_range(kv: KvSource, seq: int, start: int, end: int):
     """Token range [start, end) of sequence ``seq`` -> K, V ``[H, n, 128]``."""
