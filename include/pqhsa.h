@@ -529,12 +529,13 @@ int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t q_stride_r
  * zero).  mass f32 [B, H, mass_stride], mass_out apart from it.  n_max: a HARD bound of the lengths.
  * keep >= sink + recent; blocks as above: a row of a block outside the old cache is copied as zeros, one
  * that would go to a block outside the new one is left out.  An index of the old cache does not describe
- * the new one: it has to be encoded again.
+ * the new one: it has to be encoded again.  workspace: 256-byte aligned, used during the call only.
  */
+size_t pqhsa_evict_workspace_bytes(int32_t B, int32_t H, int32_t n_max);
 int pqhsa_evict(const pqhsa_kv_view *src, int32_t src_blocks, const pqhsa_kv_view *dst, int32_t dst_blocks,
                 int32_t B, int32_t H, const float *mass, int64_t mass_stride, const int32_t *seq_lens,
                 int32_t n_max, int32_t keep, int32_t sink, int32_t recent, int32_t *kept, int32_t *new_lens,
-                float *mass_out, int64_t mass_out_stride, void *stream);
+                float *mass_out, int64_t mass_out_stride, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
  * Paged-KV readers (benchmarks/vllm_backend/paged_kv_fa.py:95-156).  Both copy rows of

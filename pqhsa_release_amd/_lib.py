@@ -154,8 +154,10 @@ SIGNATURES = {
     "pqhsa_prompt_attend_paged": (ctypes.c_int, [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64,
                                                  c_void_p, _P(KvView), c_int32, c_int32, c_int32, c_int32, c_void_p, c_int32,
                                                  c_int32, _P(Score), c_void_p, _P(Mass), c_void_p, c_size_t, c_void_p]),
+    "pqhsa_evict_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
     "pqhsa_evict": (ctypes.c_int, [_P(KvView), c_int32, _P(KvView), c_int32, c_int32, c_int32, c_void_p, c_int64, c_void_p,
-                                   c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+                                   c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_size_t,
+                                   c_void_p]),
     "pqhsa_gather_probe": (ctypes.c_int, [_P(KvView), c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p]),
 }
 

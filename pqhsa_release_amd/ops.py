@@ -993,9 +993,11 @@ def evict(kv: KvSource, dst: KvSource, mass: torch.Tensor, seq_lens: torch.Tenso
     with _on_device(device):
         kept = torch.empty(b, h, keep, dtype=torch.int32, device=device)
         new_lens = torch.empty(b, dtype=torch.int32, device=device)
+        need = lib.pqhsa_evict_workspace_bytes(b, h, n_max)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
         rc = lib.pqhsa_evict(kv.ref(), kv.blocks, dst.ref(), dst.blocks, b, h, mass.data_ptr(), mass.shape[2],
                              seq_lens.data_ptr(), n_max, keep, int(sink), int(recent), kept.data_ptr(), new_lens.data_ptr(),
-                             _ptr(mass_out), 0 if mass_out is None else mass_out.shape[2], _stream())
+                             _ptr(mass_out), 0 if mass_out is None else mass_out.shape[2], ws.data_ptr(), need, _stream())
     _lib.check(rc, "pqhsa_evict")
     return kept, new_lens
 

@@ -120,10 +120,17 @@ def test_selection(masses, keep, sink, recent):
 
 
 @gpu
-@pytest.mark.parametrize("n", [1, 2, 1023, 1024, 16384, 16385, 50001])
+@pytest.mark.parametrize("n", [1, 2, 1023, 1024, 16383, 16384, 16385, 32768, 50001])
 def test_long_and_odd_rows(n):
     check([n], max(1, n // 3), 0 if n < 10 else 4, 0 if n < 10 else 3, masses="ties", heads=1, seed=n)
     check([n], max(1, n // 2), 0 if n < 10 else 1, 0, heads=1, seed=n + 1)
+
+
+@gpu
+@pytest.mark.parametrize("masses", ["heavy", "ties", "zero", "odd"])
+@pytest.mark.parametrize("keep,sink,recent", [(1, 0, 0), (17000, 16500, 300), (20000, 3, 16390), (34000, 40, 2)])
+def test_streams_of_several_chunks(masses, keep, sink, recent):
+    check([40000, 16385, 33000, 0, 9], keep, sink, recent, masses=masses, heads=1, layout="dense", seed=keep)
 
 
 @gpu
@@ -249,14 +256,15 @@ def test_c_entry_refuses_bad_arguments_before_any_gpu_work():
         v.k_base = v.v_base = (1 + k) << 20
         v.dtype, v.stride_tok, v.stride_head, v.stride_seq = _lib.BF16, 128, 1280, 12800
 
-    def call(B=1, H=1, n_max=10, stride=10, keep=5, sink=1, recent=1, mass=1 << 20, out=None, out_stride=0):
+    def call(B=1, H=1, n_max=10, stride=10, keep=5, sink=1, recent=1, mass=1 << 20, out=None, out_stride=0, ws=1 << 20, ws_bytes=1 << 20):
         return lib.pqhsa_evict(ctypes.byref(src), 0, ctypes.byref(dst), 0, B, H, mass, stride, 1 << 20, n_max, keep, sink, recent,
-                               1 << 20, 1 << 20, out, out_stride, None)
+                               1 << 20, 1 << 20, out, out_stride, ws, ws_bytes, None)
 
     assert call(keep=1) == -1 and call(keep=0, sink=0, recent=0) == -1 and call(sink=-1) == -1
     assert call(keep=2**31 - 1, sink=2**31 - 1, recent=2**31 - 1) == -1
     assert call(stride=9) == -1 and call(n_max=-1) == -1 and call(H=0) == -1 and call(B=70000) == -1 and call(mass=None) == -1
-    assert call(out=1 << 20, out_stride=4) == -1
+    assert call(out=1 << 20, out_stride=4) == -1 and call(ws=None) == -1 and call(ws=16) == -1
+    assert call(n_max=1 << 20, stride=1 << 20, ws_bytes=256) == -3 and b"workspace" in lib.pqhsa_last_error()
     assert call(B=0) == 0
     dst.dtype = _lib.F16
     assert call() == -1
