@@ -20,10 +20,23 @@
 
 namespace pqhsa {
 
-constexpr int kPromptThreads = 256;
-constexpr int kPromptRows = 128;       // packed rows per workgroup
-constexpr int kPromptSlots = 4;        // tiles whose row addresses are kept
-constexpr int kPromptBuffer = 32768;   // bytes of a K/V tile pair in LDS
+constexpr int KT = 32;                 // keys per tile
+
+constexpr int kPromptWaves = 4;        // 32 rows each
+constexpr int kPromptThreads = kPromptWaves * kWave;
+constexpr int kPromptRows = kPromptWaves * 32;         // packed rows per workgroup
+constexpr int kPromptFill = 768;       // workgroups that fill the chip
+constexpr int kSlots = 8;              // tiles whose row addresses are known or on their way
+
+// LDS: three K/V tiles (two in fp32) and the slots; three (two) workgroups share a compute unit.
+template <int DT>
+struct PromptShape {
+    static constexpr int kRowBytes = kD * (DT == PQHSA_F32 ? 4 : 2);
+    static constexpr int kTileBytes = KT * kRowBytes;
+    static constexpr int kStages = DT == PQHSA_F32 ? 2 : 3;
+    static constexpr int kPerCu = DT == PQHSA_F32 ? 2 : 3;
+    static constexpr int kLds = 2 * kStages * kTileBytes + kSlots * (KT * 16 + 8) + 16;
+};
 
 struct PromptArgs {
     const char *q;
@@ -40,6 +53,7 @@ struct PromptArgs {
     ScoreArgs score;
     int tiles;                         // row tiles of the launch
     int splits;
+    uint32_t block_magic;              // (2^32 - 1) / block_size
     int mask_words;                    // words of the per-tile bit mask in LDS (documents)
     float *part_o;                     // [T * H * G, splits, 128]
     float2 *part_ml;                   // [T * H * G, splits]
@@ -62,6 +76,7 @@ __device__ inline PromptRows sequence_rows(const int32_t *cu, int64_t T, int b) 
 }
 
 // The workgroup's row tile: sequence and tile number inside it (b < 0: none).  Every wave finds it by itself.
+template <int ROWS>
 __device__ inline void find_row_tile(const PromptArgs &a, int want, int &b_out, int &tile_out) {
     const int lane = threadIdx.x & 63;
     int before = 0;
@@ -69,7 +84,7 @@ __device__ inline void find_row_tile(const PromptArgs &a, int want, int &b_out, 
         int tiles = 0;
         if (base + lane < a.B) {
             const PromptRows r = sequence_rows(a.cu_rows, a.T, base + lane);
-            tiles = (int)(((int64_t)r.rows * a.G + kPromptRows - 1) / kPromptRows);
+            tiles = (int)(((int64_t)r.rows * a.G + ROWS - 1) / ROWS);
         }
         const int upto = (int)wave_prefix_u32((uint32_t)tiles);
         const uint64_t hit = __ballot(before + upto > want);
@@ -96,33 +111,73 @@ __device__ inline uint32_t finite_part(uint32_t w) {
     }
 }
 
+// 16 bytes per lane from memory into LDS at the wave-uniform byte address `lds` plus 16 * lane, without
+// passing through registers.  The compiler does not see the access: whoever reads the LDS waits with
+// direct_loads_done() and a barrier first.  (M0, which holds the LDS address, has no other use here.)
+__device__ inline void load_direct(uint32_t lds, const char *p) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p) : "memory");
+}
+__device__ inline void load_direct4(uint32_t lds, const void *p) {   // 4 bytes per lane
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p) : "memory");
+}
+// all of this wave's direct loads but the last LEFT have arrived
+template <int LEFT>
+__device__ inline void direct_loads_done() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory"); }
+
+__device__ uint4 g_zero_row;           // what lanes of a row that does not exist load
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v lds_short4v;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) float lds_float;
+
 template <int DT, bool GENERAL>
-__global__ __launch_bounds__(kPromptThreads, 2) void prompt_attend_kernel(PromptArgs a) {
+__global__ __launch_bounds__(kPromptThreads, PromptShape<DT>::kPerCu) void prompt_attend_kernel(PromptArgs a) {
+    using Shape = PromptShape<DT>;
+    constexpr int kStages = Shape::kStages, kThreads = kPromptThreads;
     constexpr bool kF32 = DT == PQHSA_F32;
-    constexpr int KT = kF32 ? 32 : 64;                   // keys per tile
-    constexpr int kTT = KT / 32;                         // matrix tiles of keys
-    constexpr int kRowBytes = kD * (kF32 ? 4 : 2);
+    constexpr int kRowBytes = Shape::kRowBytes, kTileBytes = Shape::kTileBytes;
     constexpr int kSlices = kRowBytes / 32;              // 16-byte pieces of a row per lane of a pair
     constexpr int kRowLanes = kRowBytes / 16;            // lanes that fetch one row
     constexpr int kPass = 64 / kRowLanes;                // rows a wave fetches per instruction
+    constexpr int kSteps = kF32 ? 16 : KT / 16;          // matrix instructions of the value product per 32 dims
+    constexpr int kLoads = kTileBytes / 1024 / kPromptWaves;    // instructions of a wave per K or V tile
+    constexpr int kVat = kStages * kTileBytes;           // K of stage i at i * kTileBytes, V behind all of K
     extern __shared__ __align__(16) char lds[];
-    int64_t *offs = reinterpret_cast<int64_t *>(lds + 2 * kPromptBuffer);          // [slots][64]
-    int32_t *kdoc = reinterpret_cast<int32_t *>(offs + kPromptSlots * 64);         // [slots][64]
-    uint64_t *valid = reinterpret_cast<uint64_t *>(kdoc + kPromptSlots * 64);      // [slots]
-    int32_t *poison = reinterpret_cast<int32_t *>(valid + kPromptSlots);           // [2]: an infinity or NaN was set aside
-    int32_t *doc_range = poison + 2;                                               // [2]
-    uint32_t *wanted = reinterpret_cast<uint32_t *>(doc_range + 2);                // [mask_words]
+    int64_t *offs = reinterpret_cast<int64_t *>(lds + 2 * kVat);                   // [slots][32] row addresses
+    int32_t *phys = reinterpret_cast<int32_t *>(offs + kSlots * KT);               // [slots][32] blocks as looked up
+    int32_t *kdoc = phys + kSlots * KT;                                            // [slots][32] documents
+    uint32_t *valid = reinterpret_cast<uint32_t *>(kdoc + kSlots * KT);            // [slots] rows that exist
+    int32_t *tiles = reinterpret_cast<int32_t *>(valid + kSlots);                  // [slots] tile of the walk (documents)
+    int32_t *poison = tiles + kSlots;                                              // [0]: an infinity or NaN was set aside, [1]: some row inside the sequence has no place
+    uint32_t *wanted = reinterpret_cast<uint32_t *>(poison + 4);                   // [mask_words] tiles to walk
+    uint32_t *pure = wanted + a.mask_words;                                        // [mask_words] tiles of the rows' one document
+    const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char *)lds;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid / kWave;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int n = lane & 31, kg = lane >> 5;
-    const int h = blockIdx.x, split = blockIdx.z;
+    // Workgroups go to the eight XCDs in turn: where heads and splits allow it, the row tiles of one
+    // (head, split) stay on one XCD, whose L2 then holds their K/V.
+    const int streams = a.H * a.splits;
+    int stream, order;
+    if (streams % 8 == 0) {
+        const int id = blockIdx.x / 8;
+        order = id % a.tiles;
+        stream = id / a.tiles * 8 + (int)(blockIdx.x % 8);
+    } else {
+        stream = blockIdx.x % streams;
+        order = blockIdx.x / streams;
+    }
+    const int h = stream % a.H, split = stream / a.H;
     int b, tile;
-    find_row_tile(a, a.tiles - 1 - (int)blockIdx.y, b, tile);    // the longest rows of a prompt first
+    find_row_tile<kPromptRows>(a, a.tiles - 1 - order, b, tile);      // the longest rows of a prompt first
     if (b < 0) return;
     b = __builtin_amdgcn_readfirstlane(b);
     tile = __builtin_amdgcn_readfirstlane(tile);
-    const PromptRows rows = sequence_rows(a.cu_rows, a.T, b);
-    const int len = sequence_length(a.seq_lens, b, a.n_max);
+    PromptRows rows = sequence_rows(a.cu_rows, a.T, b);
+    rows.first = __builtin_amdgcn_readfirstlane((int)rows.first);    // (T is below 2^31)
+    rows.rows = __builtin_amdgcn_readfirstlane(rows.rows);
+    const int len = __builtin_amdgcn_readfirstlane(sequence_length(a.seq_lens, b, a.n_max));
     const int first_pos = len - rows.rows;
     const int64_t packed = (int64_t)rows.rows * a.G;
     const int64_t pr = (int64_t)tile * kPromptRows + wave * 32 + n;
@@ -130,7 +185,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void prompt_attend_kernel(Prompt
     const int prc = (int)(mine ? pr : packed - 1);       // rows past the end repeat the last one
     const int token = prc / a.G, g = prc - token * a.G;
     const int pos = first_pos + token;
-    const int prefix_all = min(sequence_prefix(a.score, b), len);
+    const int prefix_all = __builtin_amdgcn_readfirstlane(min(sequence_prefix(a.score, b), len));
     // positions of the workgroup's rows, and of the wave's
     const int wg_lo = first_pos + (int)((int64_t)tile * kPromptRows / a.G);
     const int wg_hi = first_pos + (int)((min((int64_t)(tile + 1) * kPromptRows, packed) - 1) / a.G);
@@ -150,125 +205,149 @@ __global__ __launch_bounds__(kPromptThreads, 2) void prompt_attend_kernel(Prompt
     const int t_begin = min(split * per, count), t_end = min(t_begin + per, count);
     auto key_tile = [&](int t) { return (t < walk_a ? t : walk_b + t - walk_a) * KT; };
 
-    if (docs) {                                          // a bit per tile of the walk: some key of the rows' documents
-        if (tid == 0) { doc_range[0] = 0x7fffffff; doc_range[1] = -0x7fffffff - 1; }
-        for (int w = tid; w < a.mask_words; w += kPromptThreads) wanted[w] = 0u;
-        __syncthreads();
-        for (int p = max(wg_lo, 0) + tid; p <= wg_hi; p += kPromptThreads) {
-            atomicMin(&doc_range[0], docs[p]);
-            atomicMax(&doc_range[1], docs[p]);
-        }
-        __syncthreads();
-        const int d_lo = doc_range[0], d_hi = doc_range[1];
-        for (int x = tid; x < (t_end - t_begin) * KT; x += kPromptThreads) {
-            const int j = key_tile(t_begin + x / KT) + x % KT;
-            if (j < len) {
-                const int d = docs[j];
-                if (d >= d_lo && d <= d_hi) atomicOr(&wanted[x / KT / 32], 1u << (x / KT % 32));
+    if (docs && t_begin < t_end) {
+        // a bit per tile of the walk: some key lies in the rows' documents; every key is of their one document
+        int d_lo = 0x7fffffff, d_hi = -0x7fffffff - 1;
+        for (int p = max(wg_lo, 0) + lane; p <= wg_hi; p += 64) { d_lo = min(d_lo, docs[p]); d_hi = max(d_hi, docs[p]); }
+#pragma unroll
+        for (int x = 32; x > 0; x >>= 1) { d_lo = min(d_lo, __shfl_xor(d_lo, x, kWave)); d_hi = max(d_hi, __shfl_xor(d_hi, x, kWave)); }
+        for (int w = wave; w * 32 < t_end - t_begin; w += kPromptWaves) {
+            uint32_t some = 0, whole = 0;
+#pragma unroll 1
+            for (int x0 = 0; x0 < 32; x0 += 16) {
+                int d[8];
+                bool in[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {            // two tiles a load
+                    const int t = t_begin + w * 32 + x0 + 2 * x + lane / KT;
+                    const int j = key_tile(t) + lane % KT;
+                    in[x] = t < t_end && j < len;
+                    d[x] = in[x] ? docs[j] : 0;
+                }
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const uint64_t hit = __ballot(in[x] && d[x] >= d_lo && d[x] <= d_hi);
+                    const uint64_t same = __ballot(in[x] && d[x] == d_lo && d_lo == d_hi);
+                    some |= ((uint32_t)hit ? 1u : 0u) << (x0 + 2 * x) | ((hit >> 32) ? 2u : 0u) << (x0 + 2 * x);
+                    whole |= ((uint32_t)same == ~0u ? 1u : 0u) << (x0 + 2 * x) | ((uint32_t)(same >> 32) == ~0u ? 2u : 0u) << (x0 + 2 * x);
+                }
             }
+            if (lane == 0) { wanted[w] = some; pure[w] = whole; }
         }
         __syncthreads();
     }
     // the first tile at or after t that has to be walked (t_end: none)
     auto next = [&](int t) {
-        if (!docs) return t;
+        if (!docs) return min(t, t_end);
         while (t < t_end) {
             const int x = t - t_begin;
-            const uint32_t bits = wanted[x / 32] >> (x % 32);
+            const uint32_t bits = __builtin_amdgcn_readfirstlane(wanted[x / 32]) >> (x % 32);
             if (bits) return min(t + __ffs((int)bits) - 1, t_end);
             t = t_begin + (x / 32 + 1) * 32;
         }
         return t_end;
     };
+    // whether rows at positions [lo, hi] all see every key of tile t
+    auto all_see = [&](int t, int lo, int hi) {
+        const int k0 = key_tile(t), last = k0 + KT - 1;
+        const bool one_doc = !docs || ((__builtin_amdgcn_readfirstlane(pure[(t - t_begin) / 32]) >> ((t - t_begin) % 32)) & 1);
+        return one_doc && lo >= 0 && ((last <= lo && hi - k0 < window) || last < prefix_all);
+    };
 
     // query rows as the second operand: lane (n, kg) holds row n
-    uint4 qf[kSlices];
+    u32x4 qf[kSlices];
     {
         const char *p = a.q + ((rows.first + token) * a.q_row + (int64_t)(h * a.G + g) * a.q_head) * a.kv.esize;
 #pragma unroll
-        for (int u = 0; u < kSlices; ++u) qf[u] = *reinterpret_cast<const uint4 *>(p + (u * 2 + kg) * 16);
+        for (int u = 0; u < kSlices; ++u) qf[u] = *reinterpret_cast<const u32x4 *>(p + (u * 2 + kg) * 16);
+        // waited for here: inside the loop the compiler's wait would also be one for the direct loads in flight
+#pragma unroll
+        for (int u = 0; u < kSlices; ++u) asm volatile("" : "+v"(qf[u]));
     }
     const float slope2 = GENERAL && a.score.slopes ? a.score.slopes[h * a.G + g] * kLog2e : 0.0f;
     const int row_doc = docs && pos >= 0 ? docs[pos] : 0;
     const int row_prefix = pos >= 0 ? prefix_all : 0;
-    const int row_from = pos >= 0 ? max(pos - window + 1, 0) : 0;   // keys [row_from, pos] and [0, row_prefix)
+    const int row_from = pos >= 0 ? max(pos - window + 1, 0) : 0x7fffffff;   // keys [row_from, pos] and [0, row_prefix)
 
-    // addresses of a tile's rows (the first KT threads), -1: past the sequence or outside the cache
-    auto resolve = [&](int t, int slot) {
-        if (tid < 64) {
-            const int j = key_tile(t) + tid;
-            const bool in = tid < KT && j < len;
-            int64_t off = -1;
-            if (in) off = checked_row_bytes(a.kv, a.blocks, b, h, j);
-            offs[slot * 64 + tid] = off;
-            if (docs) kdoc[slot * 64 + tid] = in ? docs[j] : 0;
-            const uint64_t ok = __ballot(off >= 0);
-            if (tid == 0) valid[slot] = ok;
+    // Tile number `x` of this workgroup's own walk, t_end behind the last.
+    auto tile_at = [&](int x) { return docs ? __builtin_amdgcn_readfirstlane(tiles[x & (kSlots - 1)]) : min(t_begin + x, t_end); };
+    // Addresses of a tile's rows, -1: past the sequence, outside the cache, or no tile at all.  The blocks
+    // come from the table straight into LDS (a load into registers would make the compiler wait for every
+    // direct load in flight); two stages later they become addresses.
+    const int32_t *table = a.kv.block_table + (int64_t)b * a.kv.max_blocks;
+    auto block_of = [&](int j) {                         // j / block_size: the product is one short at most
+        int q = (int)__umulhi((uint32_t)j, a.block_magic);
+        return j - q * a.kv.block_size >= a.kv.block_size ? q + 1 : q;
+    };
+    auto look_up = [&](int x, int t) {                   // (32 lanes of one wave)
+        if (lane >= KT) return;
+        const int slot = x & (kSlots - 1);
+        const int j = key_tile(t) + lane;
+        const bool in = t < t_end && j < len;
+        if (a.kv.paged)
+            load_direct4(lds0 + 2 * kVat + kSlots * KT * 8 + slot * KT * 4,
+                         in ? static_cast<const void *>(table + block_of(j)) : &g_zero_row);
+        if (docs) {
+            load_direct4(lds0 + 2 * kVat + kSlots * KT * 12 + slot * KT * 4, in ? static_cast<const void *>(docs + j) : &g_zero_row);
+            if (lane == 0) tiles[slot] = t;
         }
     };
-    // K: four rows' pieces a thread; V: four consecutive rows (2-byte types; four passes in fp32)
-    u32x4 ks[4], vs[4];
-    auto fetch = [&](int slot) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = (wave * 4 + i) * kPass + lane / kRowLanes;
-            const int64_t off = offs[slot * 64 + r];
-            ks[i] = *reinterpret_cast<const u32x4 *>(a.kv.k_base + (off < 0 ? 0 : off) + (lane % kRowLanes) * 16);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = kF32 ? (wave * 4 + i) * kPass + lane / kRowLanes : (wave * 4 + lane / 16) * 4 + i;
-            const int64_t off = offs[slot * 64 + r];
-            const u32x4 x = *reinterpret_cast<const u32x4 *>(a.kv.v_base + (off < 0 ? 0 : off) + (lane % kRowLanes) * 16);
-            vs[i] = off < 0 ? (u32x4){0u, 0u, 0u, 0u} : x;
-        }
-    };
-    // K rows by 16-byte pieces, the piece number xored with the row; V^T (2-byte types) rows of 64 keys by
-    // dim, 16-byte slots of 8 keys (slot 2u + kg: keys 16u + 4kg + {0..3, 8..11}), xored with the dim
-    // `watch`: a tile that some rows do not see whole.  A weight of zero would not cancel an infinite or NaN
-    // value there, so these are left out of the product and come back at the end, for the rows that see them.
-    auto store = [&](int buf, bool watch) {
-        if (watch) {
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t x = finite_part<DT>(vs[i][w]);
-                    bad |= x != vs[i][w];
-                    vs[i][w] = x;
-                }
-            if (bad) poison[0] = 1;
-        }
-        char *kl = lds + buf * kPromptBuffer, *vl = kl + kPromptBuffer / 2;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = (wave * 4 + i) * kPass + lane / kRowLanes;
-            *reinterpret_cast<u32x4 *>(kl + r * kRowBytes + (((lane % kRowLanes) ^ (r & 15)) * 16)) = ks[i];
-        }
-        if constexpr (kF32) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = (wave * 4 + i) * kPass + lane / kRowLanes;
-                *reinterpret_cast<u32x4 *>(vl + r * kRowBytes + (lane % kRowLanes) * 16) = vs[i];
-            }
+    auto resolve = [&](int x, int t) {                   // (one wave, once the blocks are there)
+        const int slot = x & (kSlots - 1);
+        const int j = key_tile(t) + (lane & (KT - 1));
+        bool ok = t < t_end && j < len;
+        int64_t off = (int64_t)h * a.kv.stride_head;
+        if (a.kv.paged) {
+            const int p = phys[slot * KT + (lane & (KT - 1))];
+            ok = ok && p >= 0 && p < a.blocks;
+            off += (int64_t)p * a.kv.stride_block + (int64_t)(j - block_of(j) * a.kv.block_size) * a.kv.stride_tok;
         } else {
-            const int q4 = wave * 4 + lane / 16, i16 = lane & 15;
-            const int slot16 = (q4 >> 2) * 2 + (q4 & 1), half = (q4 >> 1) & 1;
-#pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                uint32_t w[2];
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    w[x] = __builtin_amdgcn_perm(vs[2 * x + 1][d >> 1], vs[2 * x][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
-                *reinterpret_cast<uint2 *>(vl + (i16 * 8 + d) * 128 + ((slot16 ^ ((i16 ^ d) & 7)) * 16) + half * 8) = make_uint2(w[0], w[1]);
-            }
+            off += (int64_t)b * a.kv.stride_seq + (int64_t)j * a.kv.stride_tok;
+        }
+        if (lane < KT) offs[slot * KT + lane] = ok ? off * a.kv.esize : -1;
+        const uint32_t bits = (uint32_t)__ballot(ok), inside = (uint32_t)__ballot(t < t_end && j < len);
+        if (lane == 0) {
+            valid[slot] = bits;
+            if (bits != inside) poison[1] = 1;
         }
     };
-    // whether rows at positions [lo, hi] all see keys [k0, k0 + KT)
-    auto all_see = [&](int k0, int lo, int hi) {
-        const int last = k0 + KT - 1;
-        return !docs && lo >= 0 && ((last <= lo && hi - k0 < window) || last < prefix_all);
+    // Row r of K lies with its 16-byte piece c at place c ^ (r & 15); row r of V (2-byte types) at place
+    // c ^ 2 (r & 7): the matrix operands' reads then spread over the banks.  A tile past the end is fetched
+    // as zeros, so that the number of loads in flight is always the same.
+    auto fetch = [&](const char *base, int x, uint32_t to, bool values) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));                     // (what follows from the lane is formed here, not kept in registers)
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = (wave * kLoads + i) * kPass + ln / kRowLanes;
+            const int turn = values ? (kF32 ? 0 : (r & 7) << 1) : r & 15;
+            const int64_t off = offs[(x & (kSlots - 1)) * KT + r];
+            const char *p = off < 0 ? reinterpret_cast<const char *>(&g_zero_row) : base + (off + (uint32_t)(((ln % kRowLanes) ^ turn) * 16));
+            load_direct(lds0 + to + (wave * kLoads + i) * 1024, p);
+        }
+    };
+    auto fetch_tile = [&](int x, int stage) {
+        fetch(a.kv.k_base, x, stage * kTileBytes, false);
+        fetch(a.kv.v_base, x, kVat + stage * kTileBytes, true);
+    };
+    // A tile that some rows of the workgroup do not see whole: a weight of zero would not cancel an infinite
+    // or NaN value, so these are set aside (and come back at the end, for the rows that see them).
+    auto set_aside = [&](char *vl) {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < kTileBytes / 16 / kThreads; ++i) {  // (at least one piece a thread)
+            u32x4 *p = reinterpret_cast<u32x4 *>(vl + (i * kThreads + tid) * 16);
+            const u32x4 x = *p;
+            u32x4 y;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) y[w] = finite_part<DT>(x[w]);
+            if (x[0] != y[0] || x[1] != y[1] || x[2] != y[2] || x[3] != y[3]) {
+                *p = y;
+                bad = true;
+            }
+        }
+        if (bad) poison[0] = 1;
+        __syncthreads();
     };
 
     float m = -INFINITY, l = 0.0f;
@@ -277,97 +356,67 @@ __global__ __launch_bounds__(kPromptThreads, 2) void prompt_attend_kernel(Prompt
     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[dt][r] = 0.0f;
+    // where GENERAL is false scores stay unscaled, the scale goes into the exponent
+    const float unit = GENERAL ? 1.0f : a.score.scale2;
 
-    // value product of the tile: weights in the operand registers, V^T from LDS
-    auto value_operand = [&](const char *vl, int u, int dt) {
-        if constexpr (kF32) {                            // (u: the accumulator register of the key's score)
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(vl + (8 * (u / 4) + 4 * kg + u % 4) * kRowBytes + (dt * 32 + n) * 4);
-            return make_uint4(w, 0u, 0u, 0u);
-        } else {
-            const int dim = dt * 32 + n;
-            return *reinterpret_cast<const uint4 *>(vl + dim * 128 + (((u * 2 + kg) ^ (((dim >> 3) ^ dim) & 7)) * 16));
-        }
-    };
-    auto value_mfma = [&](uint4 v, uint4 w, f32x16 o) {
-        if constexpr (kF32) return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v.x), __uint_as_float(w.x), o, 0, 0, 0);
-        else return Half16<DT>::mfma32(v, w, o);
-    };
-    constexpr int kSteps = kF32 ? 16 : KT / 16;          // matrix instructions per 32 dims
-
-    if (tid == 0) poison[0] = 0;
-    int t = next(t_begin), t1 = t < t_end ? next(t + 1) : t_end;
-    if (t < t_end) {
-        resolve(t, 0);
-        if (t1 < t_end) resolve(t1, 1);
-        __syncthreads();
-        fetch(0);
-        store(0, !all_see(key_tile(t), wg_lo, wg_hi));
-        __syncthreads();
-    }
-    for (int it = 0; t < t_end; ++it) {
-        const int slot = it & 3;
-        const char *kl = lds + (it & 1) * kPromptBuffer, *vl = kl + kPromptBuffer / 2;
-        const int t2 = t1 < t_end ? next(t1 + 1) : t_end;
-        const int k0 = key_tile(t);
-        if (t1 < t_end) fetch((it + 1) & 3);
-        if (t2 < t_end) resolve(t2, (it + 2) & 3);
-
-        f32x16 s[kTT];
+    // S^T of a tile: key 8 (r / 4) + 4 kg + r % 4 of row n in s[r]
+    // (The piece numbers differ in bits above the swizzle's: one lane address, and an exclusive or per piece.
+    // They are formed where they are used; kept in registers, they would push others out.)
+    auto score_product = [&](uint32_t kl, f32x16 &s) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const uint32_t at = kl + (uint32_t)((ln & 31) * kRowBytes + (((ln >> 5) ^ (ln & 15)) * 16));
 #pragma unroll
-        for (int T = 0; T < kTT; ++T) {
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[T][r] = 0.0f;
-            const int key = T * 32 + n;
+        for (int u = 0; u < kSlices; ++u) {
+            const u32x4 x = *(const lds_u32x4 *)(size_t)(at ^ (u * 32));
+            if constexpr (kF32) {
+                const f32x4 y = __builtin_bit_cast(f32x4, x), z = __builtin_bit_cast(f32x4, qf[u]);
 #pragma unroll
-            for (int u = 0; u < kSlices; ++u) {
-                const uint4 x = *reinterpret_cast<const uint4 *>(kl + key * kRowBytes + (((u * 2 + kg) ^ (key & 15)) * 16));
-                if constexpr (kF32) {
-                    const f32x4 y = __builtin_bit_cast(f32x4, x), z = __builtin_bit_cast(f32x4, qf[u]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) s[T] = __builtin_amdgcn_mfma_f32_32x32x2f32(y[c], z[c], s[T], 0, 0, 0);
-                } else {
-                    s[T] = Half16<DT>::mfma32(x, qf[u], s[T]);
-                }
+                for (int c = 0; c < 4; ++c) s = __builtin_amdgcn_mfma_f32_32x32x2f32(y[c], z[c], s, 0, 0, 0);
+            } else {
+                s = Half16<DT>::mfma32(__builtin_bit_cast(uint4, x), __builtin_bit_cast(uint4, qf[u]), s);
             }
         }
-        const bool whole = all_see(k0, w_lo, w_hi) && valid[slot] == (KT == 64 ? ~0ull : 0xffffffffull);
-        // scores; where GENERAL is false they stay unscaled, the scale goes into the exponent
-        const float unit = GENERAL ? 1.0f : a.score.scale2;
+    };
+    // the score rule on them: cap and bias (GENERAL), and the mask where the wave does not see the tile whole
+    auto finish_scores = [&](f32x16 &s, int t, int slot, bool holes) {
+        const int k0 = key_tile(t);
         if constexpr (GENERAL) {
 #pragma unroll
-            for (int T = 0; T < kTT; ++T)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int j = k0 + T * 32 + 8 * (r / 4) + 4 * kg + r % 4;
-                    const float x = s[T][r];
-                    s[T][r] = (a.score.capped ? a.score.cap2 * tanh_score(x * a.score.in_cap) : x * a.score.scale2)
-                              - slope2 * (float)abs(pos - j);
-                }
+            for (int r = 0; r < 16; ++r) {
+                const int j = k0 + 8 * (r / 4) + 4 * kg + r % 4;
+                s[r] = (a.score.capped ? a.score.cap2 * tanh_score(s[r] * a.score.in_cap) : s[r] * a.score.scale2) - slope2 * (float)abs(pos - j);
+            }
         }
-        if (!whole) {
-            const uint64_t ok = valid[slot] >> (4 * kg);
+        if (!holes && all_see(t, w_lo, w_hi)) return;
+        // (bitwise, not short-circuit: a branch per key costs more than the comparisons)
+        const uint32_t exist = valid[slot] >> (4 * kg);
+        uint32_t seen = 0;
 #pragma unroll
-            for (int T = 0; T < kTT; ++T)
+        for (int r4 = 0; r4 < 4; ++r4) {
+            int4 kd = make_int4(0, 0, 0, 0);
+            if (docs) kd = *reinterpret_cast<const int4 *>(&kdoc[slot * KT + 8 * r4 + 4 * kg]);
+            const int d[4] = {kd.x, kd.y, kd.z, kd.w};
 #pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4) {
-                    int4 kd = make_int4(0, 0, 0, 0);
-                    if (docs) kd = *reinterpret_cast<const int4 *>(&kdoc[slot * 64 + T * 32 + 8 * r4 + 4 * kg]);
-                    const int d[4] = {kd.x, kd.y, kd.z, kd.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int j = k0 + T * 32 + 8 * r4 + 4 * kg + e;
-                        bool see = ((j >= row_from && j <= pos) || j < row_prefix) && ((ok >> (T * 32 + 8 * r4 + e)) & 1);
-                        if (docs) see = see && d[e] == row_doc;
-                        s[T][4 * r4 + e] = see ? s[T][4 * r4 + e] : -INFINITY;
-                    }
-                }
+            for (int e = 0; e < 4; ++e) {
+                const int j = k0 + 8 * r4 + 4 * kg + e;
+                const uint32_t see = ((j >= row_from) & (j <= pos)) | (j < row_prefix);
+                seen |= (docs ? see & (d[e] == row_doc) : see) << (8 * r4 + e);
+            }
         }
-        float top = -INFINITY;
+        seen &= exist;
 #pragma unroll
-        for (int T = 0; T < kTT; ++T)
+        for (int r = 0; r < 16; ++r) s[r] = (seen >> (8 * (r / 4) + r % 4)) & 1 ? s[r] : -INFINITY;
+    };
+    auto largest = [&](const f32x16 &s) {
+        float top = s[0];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[T][r]);
-        top *= unit;
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+        return top * unit;
+    };
+    auto raise_maximum = [&](float top) {
         if (__ballot(top > m + kMaxSlack)) {
             top = fmaxf(top, __shfl_xor(top, 32, kWave));
             const float to = fmaxf(m, top);
@@ -377,42 +426,105 @@ __global__ __launch_bounds__(kPromptThreads, 2) void prompt_attend_kernel(Prompt
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt) acc[dt] *= f;
         }
+    };
+    // Weights, rounded to the value type for the product (their sum l is not): each at most half a step off,
+    // independently, no more than the output's own rounding.
+    auto weigh = [&](const f32x16 &s, uint4 (&pw)[kSteps]) {
         const float base = m == -INFINITY ? 0.0f : m;
-        float p[kTT][16];
+        float p[16];
 #pragma unroll
-        for (int T = 0; T < kTT; ++T)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                p[T][r] = exp2_fast(GENERAL ? s[T][r] - base : __builtin_fmaf(s[T][r], unit, -base));
-                l += p[T][r];
-            }
-        // weights rounded to the value type for the product (their sum l is not): each at most half a
-        // step off, independently, no more than the output's own rounding
-        uint4 pw[kSteps];
+        for (int r = 0; r < 16; ++r) {
+            p[r] = exp2_fast(GENERAL ? s[r] - base : __builtin_fmaf(s[r], unit, -base));
+            l += p[r];
+        }
 #pragma unroll
         for (int u = 0; u < kSteps; ++u) {
             if constexpr (kF32) {
-                pw[u] = make_uint4(__float_as_uint(p[0][u]), 0u, 0u, 0u);
+                pw[u] = make_uint4(__float_as_uint(p[u]), 0u, 0u, 0u);
             } else {
-                const float *x = &p[u / 2][(u % 2) * 8];
+                const float *x = &p[u * 8];
                 pw[u] = make_uint4(Half16<DT>::pack(x[0], x[1]), Half16<DT>::pack(x[2], x[3]), Half16<DT>::pack(x[4], x[5]), Half16<DT>::pack(x[6], x[7]));
             }
         }
+    };
+    // O^T += V^T P.  2-byte types: a transposing read gives a lane four keys of its dim; two of them are the
+    // eight keys 16u + 4kg + {0..3, 8..11} whose weights the lane holds in pw[u].
+    auto value_product = [&](uint32_t vl, const uint4 (&pw)[kSteps]) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int vkey = 4 * (ln >> 5) + ((ln & 15) >> 2), vpiece = ((ln >> 4) & 1) * 2 + ((ln & 3) >> 1);
+        const uint32_t at = vl + (kF32 ? (uint32_t)((ln >> 5) * 4 * kRowBytes + (ln & 31) * 4)
+                                       : (uint32_t)(vkey * kRowBytes + (vpiece ^ ((vkey & 7) << 1)) * 16 + (ln & 1) * 8));
 #pragma unroll
         for (int u = 0; u < kSteps; ++u)
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt) acc[dt] = value_mfma(value_operand(vl, u, dt), pw[u], acc[dt]);
-        if (t1 < t_end) store((it + 1) & 1, !all_see(key_tile(t1), wg_lo, wg_hi));
+            for (int dt = 0; dt < 4; ++dt) {
+                if constexpr (kF32) {
+                    const float v = *(const lds_float *)(size_t)(at + (8 * (u / 4) + u % 4) * kRowBytes + dt * 128);
+                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, __uint_as_float(pw[u].x), acc[dt], 0, 0, 0);
+                } else {
+                    const uint32_t p = (at ^ (dt * 64)) + u * 16 * kRowBytes;
+                    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v *)(size_t)p));
+                    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v *)(size_t)(p + 8 * kRowBytes)));
+                    acc[dt] = Half16<DT>::mfma32(make_uint4(x.x, x.y, y.x, y.y), pw[u], acc[dt]);
+                }
+            }
+    };
+
+    // The pipeline: tile x is computed, tile x + stages - 1 requested, the rows of the one behind it turned into
+    // addresses, the blocks of two more looked up; a barrier per tile.  The overlap of matrix products,
+    // softmax and LDS reads is between the workgroups that share the compute unit.
+    constexpr int kInFlight = (kStages - 2) * 2 * kLoads;
+    constexpr int kAhead = kStages - 1;                  // tiles between a fetch and its use
+    if (tid == 0) { poison[0] = 0; poison[1] = 0; }
+    int t = next(t_begin), reach = t;
+    if (t < t_end) {
         __syncthreads();
-        t = t1;
-        t1 = t2;
+        for (int x = 0, at = t; x < kAhead + 3; ++x) {   // the first slots, in turn by the waves
+            if (x % kPromptWaves == wave) look_up(x, at);
+            reach = at;
+            at = next(at + 1);
+        }
+        direct_loads_done<0>();
+        __syncthreads();
+        for (int x = wave; x <= kAhead; x += kPromptWaves) resolve(x, tile_at(x));
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) fetch_tile(x, x);
+        direct_loads_done<kInFlight>();
+        __syncthreads();
+        if (!all_see(t, wg_lo, wg_hi)) set_aside(lds + kVat);
     }
+    int stage = 0;
+#pragma unroll 1
+    for (int x = 0; t < t_end; ++x) {
+        const bool holes = __builtin_amdgcn_readfirstlane(poison[1]);
+        fetch_tile(x + kAhead, stage == 0 ? kAhead : stage - 1);
+        if (docs) reach = next(reach + 1);
+        if (wave == (x & 3)) look_up(x + kAhead + 3, docs ? reach : min(t_begin + x + kAhead + 3, t_end));
+        if (wave == ((x + 2) & 3)) resolve(x + kAhead + 1, tile_at(x + kAhead + 1));
+        f32x16 s;
+        uint4 pw[kSteps];
+        score_product(lds0 + stage * kTileBytes, s);
+        finish_scores(s, t, x & (kSlots - 1), holes);
+        raise_maximum(largest(s));
+        weigh(s, pw);
+        value_product(lds0 + kVat + stage * kTileBytes, pw);
+        t = tile_at(x + 1);
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        if (t < t_end) {
+            direct_loads_done<kInFlight>();
+            __syncthreads();
+            if (!all_see(t, wg_lo, wg_hi)) set_aside(lds + kVat + stage * kTileBytes);
+        }
+    }
+    direct_loads_done<0>();                              // (no load may reach the LDS after the workgroup has left it)
     l += __shfl_xor(l, 32, kWave);
     if (t_begin < t_end && poison[0]) {                  // the infinities and NaN that were set aside
 #pragma unroll 1
         for (t = next(t_begin); t < t_end; t = next(t + 1)) {
             const int k0 = key_tile(t);
-            if (all_see(k0, wg_lo, wg_hi)) continue;
+            if (all_see(t, wg_lo, wg_hi)) continue;
 #pragma unroll 1
             for (int j = k0; j < min(k0 + KT, len); ++j) {
                 const int64_t off = checked_row_bytes(a.kv, a.blocks, b, h, j);
@@ -465,7 +577,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void prompt_attend_kernel(Prompt
 // keys as the first operand in registers and walks the counted rows; every lane sums its rows' weights
 // of 16 keys, the lanes are summed at the end: no atomics, one owner per key.
 template <int DT>
-__global__ __launch_bounds__(kPromptThreads, 2) void prompt_mass_kernel(PromptArgs a) {
+__global__ __launch_bounds__(256, 2) void prompt_mass_kernel(PromptArgs a) {
     constexpr bool kF32 = DT == PQHSA_F32;
     constexpr int kSlices = kD * (kF32 ? 4 : 2) / 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid / kWave;
@@ -560,18 +672,18 @@ struct PromptPlan {
     size_t ml_at, lse_at, bytes;
 };
 
-PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint, int key_tile, bool own_lse) {
+PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint, bool own_lse) {
     PromptPlan p = {};
-    p.tiles = (T * G + kPromptRows - 1) / kPromptRows + B;          // every sequence may end inside a tile
+    p.tiles = (T * G + kPromptRows - 1) / kPromptRows + B;              // every sequence may end inside a tile
     int64_t busy = p.tiles - B;
     if (rows_hint > 0 && rows_hint * (int64_t)B <= T) {             // about as many tiles as sequences have
         const int64_t each = ((int64_t)rows_hint * G + kPromptRows - 1) / kPromptRows;
         if (each * B > busy) busy = each * B;
     }
     if (busy < 1) busy = 1;
-    // two workgroups per compute unit, at least four key tiles each
-    const int64_t want = (512 + busy * H - 1) / (busy * H);
-    const int64_t most = ((int64_t)n_max + 4 * key_tile - 1) / (4 * key_tile);
+    // fill the chip, with at least four key tiles a workgroup
+    const int64_t want = (kPromptFill + busy * H - 1) / (busy * H);
+    const int64_t most = ((int64_t)n_max + 255) / 256;
     p.splits = (int)(want < most ? want : most);
     if (p.splits < 1) p.splits = 1;
     const size_t rows = (size_t)T * H * G;
@@ -587,14 +699,15 @@ PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint,
 }
 
 template <int DT, bool GENERAL>
-int launch_prompt(const PromptArgs &a, size_t lds, hipStream_t stream) {
+int launch_prompt(const PromptArgs &a, hipStream_t stream) {
     auto kern = prompt_attend_kernel<DT, GENERAL>;
+    const size_t lds = PromptShape<DT>::kLds + 2 * (size_t)a.mask_words * 4;
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) {
         set_error("prompt_attend: cannot raise the LDS limit to %zu: %s", lds, hipGetErrorString(e));
         return PQHSA_ELAUNCH;
     }
-    hipLaunchKernelGGL(kern, dim3((unsigned)a.H, (unsigned)a.tiles, (unsigned)a.splits), dim3(kPromptThreads), lds, stream, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.H * a.tiles * a.splits)), dim3(kPromptThreads), lds, stream, a);
     return check_launch("prompt_attend");
 }
 
@@ -607,7 +720,7 @@ using namespace pqhsa;
 extern "C" size_t pqhsa_prompt_attend_workspace_bytes(int64_t T, int32_t B, int32_t H, int32_t G, int32_t n_max,
                                                       int32_t rows_hint, int32_t dtype, int32_t with_lse) {
     if (T <= 0 || B <= 0 || H <= 0 || G <= 0 || n_max <= 0) return 256;
-    const size_t need = plan_prompt(T, B, H, G, n_max, rows_hint, dtype == PQHSA_F32 ? 32 : 64, with_lse == 0).bytes;
+    const size_t need = plan_prompt(T, B, H, G, n_max, rows_hint, with_lse == 0).bytes;
     return need < 256 ? 256 : need;
 }
 
@@ -640,9 +753,8 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
                       "%s: %d blocks, and a table of %d x %d tokens for n_max %d", what, blocks, kv->max_blocks, kv->block_size, n_max);
     PQHSA_REQUIRE(T * G < 0x7fffffff && T * H * G < 0x7fffffff, "%s: %lld rows of %d x %d heads are too many", what, (long long)T, H, G);
     PQHSA_REQUIRE((int64_t)B * H <= 65535, "%s: too many sequences and heads", what);
-    const int key_tile = kv->dtype == PQHSA_F32 ? 32 : 64;
-    const PromptPlan p = plan_prompt(T, B, H, G, n_max, rows_hint, key_tile, lse == nullptr);
-    PQHSA_REQUIRE(p.tiles <= 65535 && p.splits <= 65535, "%s: %lld row tiles are too many for one launch", what, (long long)p.tiles);
+        const PromptPlan p = plan_prompt(T, B, H, G, n_max, rows_hint, lse == nullptr);
+    PQHSA_REQUIRE(p.tiles * H * p.splits <= 0x7fffffff, "%s: %lld row tiles are too many for one launch", what, (long long)p.tiles);
     if (workspace_bytes < p.bytes) {
         set_error("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, p.bytes);
         return PQHSA_ENOSPC;
@@ -657,15 +769,16 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
     a.blocks = blocks; a.B = B; a.H = H; a.G = G; a.cu_rows = cu_rows; a.T = T; a.seq_lens = seq_lens; a.n_max = n_max;
     a.score = make_score(score);
     a.tiles = (int)p.tiles;
+    a.block_magic = kv->paged ? 0xffffffffu / (uint32_t)kv->block_size : 0u;
     a.splits = p.splits;
-    a.mask_words = score->docs ? (n_max / key_tile + 2 + 31) / 32 + 1 : 0;
+    a.mask_words = score->docs ? (n_max / KT + 2 + 31) / 32 + 1 : 0;
     a.part_o = reinterpret_cast<float *>(w);
     a.part_ml = reinterpret_cast<float2 *>(w + p.ml_at);
-    const size_t lds = 2 * kPromptBuffer + kPromptSlots * (64 * 8 + 64 * 4 + 8) + 16 + (size_t)a.mask_words * 4;
-    PQHSA_REQUIRE(lds <= 160 * 1024, "%s: n_max %d too large for a document mask", what, n_max);
+    const size_t most_lds = PromptShape<PQHSA_F32>::kLds + 2 * (size_t)a.mask_words * 4;
+    PQHSA_REQUIRE(most_lds <= 160 * 1024, "%s: n_max %d too large for a document mask", what, n_max);
     if (T > 0) {
         const bool general = score->softcap > 0.0f || score->slopes || !(score->scale > 0.0f);
-        PQHSA_DISPATCH_DTYPE(kv->dtype, rc = general ? launch_prompt<DT, true>(a, lds, stream) : launch_prompt<DT, false>(a, lds, stream));
+        PQHSA_DISPATCH_DTYPE(kv->dtype, rc = general ? launch_prompt<DT, true>(a, stream) : launch_prompt<DT, false>(a, stream));
         if (rc) return rc;
         if (p.splits > 1) {
             JoinArgs j = {a.part_o, a.part_ml, p.splits, H * G, a.out, a.out_row, a.out_head, a.lse, cu_rows + B};
@@ -676,7 +789,7 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
     if (mass && n_max > 0) {
         a.mass_in = mass->in; a.mass_out = mass->out; a.mass_stride = mass->stride; a.decay = mass->decay; a.mass_rows = mass->rows;
         const dim3 grid((unsigned)((n_max + 127) / 128), (unsigned)(B * H));
-        PQHSA_DISPATCH_DTYPE(kv->dtype, hipLaunchKernelGGL(prompt_mass_kernel<DT>, grid, dim3(kPromptThreads), 0, stream, a));
+        PQHSA_DISPATCH_DTYPE(kv->dtype, hipLaunchKernelGGL(prompt_mass_kernel<DT>, grid, dim3(256), 0, stream, a));
         rc = check_launch("prompt_mass");
     }
     return rc;
