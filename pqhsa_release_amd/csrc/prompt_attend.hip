@@ -20,22 +20,17 @@
 
 namespace pqhsa {
 
-constexpr int KT = 32;                 // keys per tile
+constexpr int kTileBytes = 16384;      // a K or V tile in LDS
 
-constexpr int kPromptWaves = 4;        // 32 rows each
-constexpr int kPromptThreads = kPromptWaves * kWave;
-constexpr int kPromptRows = kPromptWaves * 32;         // packed rows per workgroup
-constexpr int kPromptFill = 768;       // workgroups that fill the chip
-constexpr int kSlots = 8;              // tiles whose row addresses are known or on their way
-
-// LDS: three K/V tiles (two in fp32) and the slots; three (two) workgroups share a compute unit.
-template <int DT>
+// Two shapes of workgroup (32 rows a wave either way).
+template <int WAVES>
 struct PromptShape {
-    static constexpr int kRowBytes = kD * (DT == PQHSA_F32 ? 4 : 2);
-    static constexpr int kTileBytes = KT * kRowBytes;
-    static constexpr int kStages = DT == PQHSA_F32 ? 2 : 3;
-    static constexpr int kPerCu = DT == PQHSA_F32 ? 2 : 3;
-    static constexpr int kLds = 2 * kStages * kTileBytes + kSlots * (KT * 16 + 8) + 16;
+    static constexpr int kWaves = WAVES;
+    static constexpr int kThreads = WAVES * kWave;
+    static constexpr int kRows = WAVES * 32;             // packed rows
+    static constexpr int kStages = WAVES / 2;            // K/V tiles in LDS
+    static constexpr int kSlots = 2 * kStages;           // tiles whose row addresses are known or on their way
+    static constexpr int kLds = 2 * kStages * kTileBytes + kSlots * (64 * 8 + 64 * 4 + 64 * 4 + 8 + 4) + 16;
 };
 
 struct PromptArgs {
@@ -128,28 +123,28 @@ __device__ uint4 g_zero_row;           // what lanes of a row that does not exis
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v lds_short4v;
-typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-typedef __attribute__((address_space(3))) float lds_float;
 
-template <int DT, bool GENERAL>
-__global__ __launch_bounds__(kPromptThreads, PromptShape<DT>::kPerCu) void prompt_attend_kernel(PromptArgs a) {
-    using Shape = PromptShape<DT>;
-    constexpr int kStages = Shape::kStages, kThreads = kPromptThreads;
+template <int DT, bool GENERAL, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_attend_kernel(PromptArgs a) {
+    using Shape = PromptShape<WAVES>;
+    constexpr int kStages = Shape::kStages, kSlots = Shape::kSlots, kPromptRows = Shape::kRows, kThreads = Shape::kThreads;
     constexpr bool kF32 = DT == PQHSA_F32;
-    constexpr int kRowBytes = Shape::kRowBytes, kTileBytes = Shape::kTileBytes;
+    constexpr int KT = kF32 ? 32 : 64;                   // keys per tile
+    constexpr int kTT = KT / 32;                         // matrix tiles of keys
+    constexpr int kRowBytes = kD * (kF32 ? 4 : 2);
     constexpr int kSlices = kRowBytes / 32;              // 16-byte pieces of a row per lane of a pair
     constexpr int kRowLanes = kRowBytes / 16;            // lanes that fetch one row
     constexpr int kPass = 64 / kRowLanes;                // rows a wave fetches per instruction
     constexpr int kSteps = kF32 ? 16 : KT / 16;          // matrix instructions of the value product per 32 dims
-    constexpr int kLoads = kTileBytes / 1024 / kPromptWaves;    // instructions of a wave per K or V tile
+    constexpr int kLoads = 16 / WAVES;                   // instructions of a wave per K or V tile
     constexpr int kVat = kStages * kTileBytes;           // K of stage i at i * kTileBytes, V behind all of K
     extern __shared__ __align__(16) char lds[];
-    int64_t *offs = reinterpret_cast<int64_t *>(lds + 2 * kVat);                   // [slots][32] row addresses
-    int32_t *phys = reinterpret_cast<int32_t *>(offs + kSlots * KT);               // [slots][32] blocks as looked up
-    int32_t *kdoc = phys + kSlots * KT;                                            // [slots][32] documents
-    uint32_t *valid = reinterpret_cast<uint32_t *>(kdoc + kSlots * KT);            // [slots] rows that exist
+    int64_t *offs = reinterpret_cast<int64_t *>(lds + 2 * kVat);                   // [slots][64] row addresses
+    int32_t *phys = reinterpret_cast<int32_t *>(offs + kSlots * 64);               // [slots][64] blocks as looked up
+    int32_t *kdoc = phys + kSlots * 64;                                            // [slots][64] documents
+    uint64_t *valid = reinterpret_cast<uint64_t *>(kdoc + kSlots * 64);            // [slots] rows that exist
     int32_t *tiles = reinterpret_cast<int32_t *>(valid + kSlots);                  // [slots] tile of the walk (documents)
-    int32_t *poison = tiles + kSlots;                                              // [0]: an infinity or NaN was set aside, [1]: some row inside the sequence has no place
+    int32_t *poison = tiles + kSlots;                                              // [2]: an infinity or NaN was set aside
     uint32_t *wanted = reinterpret_cast<uint32_t *>(poison + 4);                   // [mask_words] tiles to walk
     uint32_t *pure = wanted + a.mask_words;                                        // [mask_words] tiles of the rows' one document
     const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char *)lds;
@@ -211,25 +206,31 @@ __global__ __launch_bounds__(kPromptThreads, PromptShape<DT>::kPerCu) void promp
         for (int p = max(wg_lo, 0) + lane; p <= wg_hi; p += 64) { d_lo = min(d_lo, docs[p]); d_hi = max(d_hi, docs[p]); }
 #pragma unroll
         for (int x = 32; x > 0; x >>= 1) { d_lo = min(d_lo, __shfl_xor(d_lo, x, kWave)); d_hi = max(d_hi, __shfl_xor(d_hi, x, kWave)); }
-        for (int w = wave; w * 32 < t_end - t_begin; w += kPromptWaves) {
+        constexpr int kPer = 64 / KT;                    // tiles a wave looks at per load
+        constexpr uint64_t kAll = KT == 64 ? ~0ull : 0xffffffffull;
+        for (int w = wave; w * 32 < t_end - t_begin; w += WAVES) {
             uint32_t some = 0, whole = 0;
 #pragma unroll 1
             for (int x0 = 0; x0 < 32; x0 += 16) {
-                int d[8];
-                bool in[8];
+                int d[16 / kPer];
+                bool in[16 / kPer];
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {            // two tiles a load
-                    const int t = t_begin + w * 32 + x0 + 2 * x + lane / KT;
+                for (int x = 0; x < 16 / kPer; ++x) {
+                    const int t = t_begin + w * 32 + x0 + x * kPer + lane / KT;
                     const int j = key_tile(t) + lane % KT;
                     in[x] = t < t_end && j < len;
                     d[x] = in[x] ? docs[j] : 0;
                 }
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
+                for (int x = 0; x < 16 / kPer; ++x) {
                     const uint64_t hit = __ballot(in[x] && d[x] >= d_lo && d[x] <= d_hi);
                     const uint64_t same = __ballot(in[x] && d[x] == d_lo && d_lo == d_hi);
-                    some |= ((uint32_t)hit ? 1u : 0u) << (x0 + 2 * x) | ((hit >> 32) ? 2u : 0u) << (x0 + 2 * x);
-                    whole |= ((uint32_t)same == ~0u ? 1u : 0u) << (x0 + 2 * x) | ((uint32_t)(same >> 32) == ~0u ? 2u : 0u) << (x0 + 2 * x);
+#pragma unroll
+                    for (int y = 0; y < kPer; ++y) {
+                        const int bit = x0 + x * kPer + y;
+                        if ((hit >> (y * 32)) & kAll) some |= 1u << bit;
+                        if (((same >> (y * 32)) & kAll) == kAll) whole |= 1u << bit;
+                    }
                 }
             }
             if (lane == 0) { wanted[w] = some; pure[w] = whole; }
@@ -247,11 +248,25 @@ __global__ __launch_bounds__(kPromptThreads, PromptShape<DT>::kPerCu) void promp
         }
         return t_end;
     };
-    // whether rows at positions [lo, hi] all see every key of tile t
-    auto all_see = [&](int t, int lo, int hi) {
-        const int k0 = key_tile(t), last = k0 + KT - 1;
+    // Tiles whose every key rows at positions [lo, hi] all see (one document aside): numbers [0, pre) and
+    // [from, to) of the walk.
+    struct Whole { int pre, from, to; };
+    auto whole_tiles = [&](int lo, int hi) {
+        Whole w = {0, 0, 0};
+        if (lo < 0) return w;
+        w.pre = min(prefix_all / KT, walk_a);            // tiles that end inside the prefix
+        const int last = (lo + 1) / KT;                  // key tiles that end at or before lo
+        const int start = a.score.window > 0 ? (max(hi - window + 1, 0) + KT - 1) / KT : 0;   // the first that begins inside hi's window
+        // key tile k is number k below walk_a, walk_a + k - walk_b from walk_b on, and in neither part between them
+        auto number = [&](int k) { return k < walk_a ? k : walk_a + max(k - walk_b, 0); };
+        w.from = number(start);
+        w.to = number(last);
+        return w;
+    };
+    const Whole wave_whole = whole_tiles(w_lo, w_hi), wg_whole = whole_tiles(wg_lo, wg_hi);
+    auto all_see = [&](int t, const Whole &w) {
         const bool one_doc = !docs || ((__builtin_amdgcn_readfirstlane(pure[(t - t_begin) / 32]) >> ((t - t_begin) % 32)) & 1);
-        return one_doc && lo >= 0 && ((last <= lo && hi - k0 < window) || last < prefix_all);
+        return one_doc && (t < w.pre || (t >= w.from && t < w.to));
     };
 
     // query rows as the second operand: lane (n, kg) holds row n
@@ -279,63 +294,55 @@ __global__ __launch_bounds__(kPromptThreads, PromptShape<DT>::kPerCu) void promp
         int q = (int)__umulhi((uint32_t)j, a.block_magic);
         return j - q * a.kv.block_size >= a.kv.block_size ? q + 1 : q;
     };
-    auto look_up = [&](int x, int t) {                   // (32 lanes of one wave)
-        if (lane >= KT) return;
+    auto look_up = [&](int x, int t) {                   // (one wave)
         const int slot = x & (kSlots - 1);
         const int j = key_tile(t) + lane;
-        const bool in = t < t_end && j < len;
+        const bool in = t < t_end && lane < KT && j < len;
         if (a.kv.paged)
-            load_direct4(lds0 + 2 * kVat + kSlots * KT * 8 + slot * KT * 4,
+            load_direct4(lds0 + 2 * kVat + kSlots * 512 + slot * 256,
                          in ? static_cast<const void *>(table + block_of(j)) : &g_zero_row);
         if (docs) {
-            load_direct4(lds0 + 2 * kVat + kSlots * KT * 12 + slot * KT * 4, in ? static_cast<const void *>(docs + j) : &g_zero_row);
+            load_direct4(lds0 + 2 * kVat + kSlots * 768 + slot * 256, in ? static_cast<const void *>(docs + j) : &g_zero_row);
             if (lane == 0) tiles[slot] = t;
         }
     };
     auto resolve = [&](int x, int t) {                   // (one wave, once the blocks are there)
         const int slot = x & (kSlots - 1);
-        const int j = key_tile(t) + (lane & (KT - 1));
-        bool ok = t < t_end && j < len;
+        const int j = key_tile(t) + lane;
+        bool ok = t < t_end && lane < KT && j < len;
         int64_t off = (int64_t)h * a.kv.stride_head;
         if (a.kv.paged) {
-            const int p = phys[slot * KT + (lane & (KT - 1))];
+            const int p = phys[slot * 64 + lane];
             ok = ok && p >= 0 && p < a.blocks;
             off += (int64_t)p * a.kv.stride_block + (int64_t)(j - block_of(j) * a.kv.block_size) * a.kv.stride_tok;
         } else {
             off += (int64_t)b * a.kv.stride_seq + (int64_t)j * a.kv.stride_tok;
         }
-        if (lane < KT) offs[slot * KT + lane] = ok ? off * a.kv.esize : -1;
-        const uint32_t bits = (uint32_t)__ballot(ok), inside = (uint32_t)__ballot(t < t_end && j < len);
-        if (lane == 0) {
-            valid[slot] = bits;
-            if (bits != inside) poison[1] = 1;
-        }
+        offs[slot * 64 + lane] = ok ? off * a.kv.esize : -1;
+        const uint64_t bits = __ballot(ok);
+        if (lane == 0) valid[slot] = bits;
     };
     // Row r of K lies with its 16-byte piece c at place c ^ (r & 15); row r of V (2-byte types) at place
     // c ^ 2 (r & 7): the matrix operands' reads then spread over the banks.  A tile past the end is fetched
     // as zeros, so that the number of loads in flight is always the same.
     auto fetch = [&](const char *base, int x, uint32_t to, bool values) {
-        int ln = lane;
-        asm volatile("" : "+v"(ln));                     // (what follows from the lane is formed here, not kept in registers)
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int r = (wave * kLoads + i) * kPass + ln / kRowLanes;
+            const int r = (wave * kLoads + i) * kPass + lane / kRowLanes;
             const int turn = values ? (kF32 ? 0 : (r & 7) << 1) : r & 15;
-            const int64_t off = offs[(x & (kSlots - 1)) * KT + r];
-            const char *p = off < 0 ? reinterpret_cast<const char *>(&g_zero_row) : base + (off + (uint32_t)(((ln % kRowLanes) ^ turn) * 16));
+            const int64_t off = offs[(x & (kSlots - 1)) * 64 + r];
+            const char *p = off < 0 ? reinterpret_cast<const char *>(&g_zero_row) : base + off + ((lane % kRowLanes) ^ turn) * 16;
             load_direct(lds0 + to + (wave * kLoads + i) * 1024, p);
         }
     };
-    auto fetch_tile = [&](int x, int stage) {
-        fetch(a.kv.k_base, x, stage * kTileBytes, false);
-        fetch(a.kv.v_base, x, kVat + stage * kTileBytes, true);
-    };
+    auto fetch_keys = [&](int x) { fetch(a.kv.k_base, x, (x & (kStages - 1)) * kTileBytes, false); };
+    auto fetch_values = [&](int x) { fetch(a.kv.v_base, x, kVat + (x & (kStages - 1)) * kTileBytes, true); };
     // A tile that some rows of the workgroup do not see whole: a weight of zero would not cancel an infinite
     // or NaN value, so these are set aside (and come back at the end, for the rows that see them).
     auto set_aside = [&](char *vl) {
         bool bad = false;
 #pragma unroll
-        for (int i = 0; i < kTileBytes / 16 / kThreads; ++i) {  // (at least one piece a thread)
+        for (int i = 0; i < kTileBytes / 16 / kThreads; ++i) {
             u32x4 *p = reinterpret_cast<u32x4 *>(vl + (i * kThreads + tid) * 16);
             const u32x4 x = *p;
             u32x4 y;
@@ -359,61 +366,71 @@ __global__ __launch_bounds__(kPromptThreads, PromptShape<DT>::kPerCu) void promp
     // where GENERAL is false scores stay unscaled, the scale goes into the exponent
     const float unit = GENERAL ? 1.0f : a.score.scale2;
 
-    // S^T of a tile: key 8 (r / 4) + 4 kg + r % 4 of row n in s[r]
-    // (The piece numbers differ in bits above the swizzle's: one lane address, and an exclusive or per piece.
-    // They are formed where they are used; kept in registers, they would push others out.)
-    auto score_product = [&](uint32_t kl, f32x16 &s) {
-        int ln = lane;
-        asm volatile("" : "+v"(ln));
-        const uint32_t at = kl + (uint32_t)((ln & 31) * kRowBytes + (((ln >> 5) ^ (ln & 15)) * 16));
+    // S^T of a tile: key 32 T + 8 (r / 4) + 4 kg + r % 4 of row n in s[T][r]
+    auto score_product = [&](const char *kl, f32x16 (&s)[kTT]) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+        for (int T = 0; T < kTT; ++T)
 #pragma unroll
-        for (int u = 0; u < kSlices; ++u) {
-            const u32x4 x = *(const lds_u32x4 *)(size_t)(at ^ (u * 32));
-            if constexpr (kF32) {
-                const f32x4 y = __builtin_bit_cast(f32x4, x), z = __builtin_bit_cast(f32x4, qf[u]);
+            for (int r = 0; r < 16; ++r) s[T][r] = 0.0f;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s = __builtin_amdgcn_mfma_f32_32x32x2f32(y[c], z[c], s, 0, 0, 0);
-            } else {
-                s = Half16<DT>::mfma32(__builtin_bit_cast(uint4, x), __builtin_bit_cast(uint4, qf[u]), s);
+        for (int u = 0; u < kSlices; ++u)
+#pragma unroll
+            for (int T = 0; T < kTT; ++T) {
+                const int key = T * 32 + n;
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(kl + key * kRowBytes + (((u * 2 + kg) ^ (n & 15)) * 16));
+                if constexpr (kF32) {
+                    const f32x4 y = __builtin_bit_cast(f32x4, x), z = __builtin_bit_cast(f32x4, qf[u]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) s[T] = __builtin_amdgcn_mfma_f32_32x32x2f32(y[c], z[c], s[T], 0, 0, 0);
+                } else {
+                    s[T] = Half16<DT>::mfma32(__builtin_bit_cast(uint4, x), __builtin_bit_cast(uint4, qf[u]), s[T]);
+                }
             }
-        }
     };
     // the score rule on them: cap and bias (GENERAL), and the mask where the wave does not see the tile whole
-    auto finish_scores = [&](f32x16 &s, int t, int slot, bool holes) {
+    auto finish_scores = [&](f32x16 (&s)[kTT], int t, int slot) {
         const int k0 = key_tile(t);
         if constexpr (GENERAL) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int j = k0 + 8 * (r / 4) + 4 * kg + r % 4;
-                s[r] = (a.score.capped ? a.score.cap2 * tanh_score(s[r] * a.score.in_cap) : s[r] * a.score.scale2) - slope2 * (float)abs(pos - j);
-            }
+            for (int T = 0; T < kTT; ++T)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = k0 + T * 32 + 8 * (r / 4) + 4 * kg + r % 4;
+                    const float x = s[T][r];
+                    s[T][r] = (a.score.capped ? a.score.cap2 * tanh_score(x * a.score.in_cap) : x * a.score.scale2)
+                              - slope2 * (float)abs(pos - j);
+                }
         }
-        if (!holes && all_see(t, w_lo, w_hi)) return;
+        const uint64_t exist = valid[slot];
+        if (all_see(t, wave_whole) && exist == (KT == 64 ? ~0ull : 0xffffffffull)) return;
         // (bitwise, not short-circuit: a branch per key costs more than the comparisons)
-        const uint32_t exist = valid[slot] >> (4 * kg);
-        uint32_t seen = 0;
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-            int4 kd = make_int4(0, 0, 0, 0);
-            if (docs) kd = *reinterpret_cast<const int4 *>(&kdoc[slot * KT + 8 * r4 + 4 * kg]);
-            const int d[4] = {kd.x, kd.y, kd.z, kd.w};
+        for (int T = 0; T < kTT; ++T) {
+            const uint32_t ok = (uint32_t)(exist >> (32 * T)) >> (4 * kg);
+            uint32_t seen = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int j = k0 + 8 * r4 + 4 * kg + e;
-                const uint32_t see = ((j >= row_from) & (j <= pos)) | (j < row_prefix);
-                seen |= (docs ? see & (d[e] == row_doc) : see) << (8 * r4 + e);
+            for (int r4 = 0; r4 < 4; ++r4) {
+                int4 kd = make_int4(0, 0, 0, 0);
+                if (docs) kd = *reinterpret_cast<const int4 *>(&kdoc[slot * 64 + T * 32 + 8 * r4 + 4 * kg]);
+                const int d[4] = {kd.x, kd.y, kd.z, kd.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int j = k0 + T * 32 + 8 * r4 + 4 * kg + e;
+                    const uint32_t see = ((j >= row_from) & (j <= pos)) | (j < row_prefix);
+                    seen |= (docs ? see & (d[e] == row_doc) : see) << (8 * r4 + e);
+                }
             }
+            seen &= ok;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[T][r] = (seen >> (8 * (r / 4) + r % 4)) & 1 ? s[T][r] : -INFINITY;
         }
-        seen &= exist;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = (seen >> (8 * (r / 4) + r % 4)) & 1 ? s[r] : -INFINITY;
     };
-    auto largest = [&](const f32x16 &s) {
-        float top = s[0];
+    auto largest = [&](const f32x16 (&s)[kTT]) {
+        float top = -INFINITY;
 #pragma unroll
-        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+        for (int T = 0; T < kTT; ++T)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[T][r]);
         return top * unit;
     };
     auto raise_maximum = [&](float top) {
@@ -429,20 +446,22 @@ __global__ __launch_bounds__(kPromptThreads, PromptShape<DT>::kPerCu) void promp
     };
     // Weights, rounded to the value type for the product (their sum l is not): each at most half a step off,
     // independently, no more than the output's own rounding.
-    auto weigh = [&](const f32x16 &s, uint4 (&pw)[kSteps]) {
+    auto weigh = [&](const f32x16 (&s)[kTT], uint4 (&pw)[kSteps]) {
         const float base = m == -INFINITY ? 0.0f : m;
-        float p[16];
+        float p[kTT][16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            p[r] = exp2_fast(GENERAL ? s[r] - base : __builtin_fmaf(s[r], unit, -base));
-            l += p[r];
-        }
+        for (int T = 0; T < kTT; ++T)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                p[T][r] = exp2_fast(GENERAL ? s[T][r] - base : __builtin_fmaf(s[T][r], unit, -base));
+                l += p[T][r];
+            }
 #pragma unroll
         for (int u = 0; u < kSteps; ++u) {
             if constexpr (kF32) {
-                pw[u] = make_uint4(__float_as_uint(p[u]), 0u, 0u, 0u);
+                pw[u] = make_uint4(__float_as_uint(p[0][u]), 0u, 0u, 0u);
             } else {
-                const float *x = &p[u * 8];
+                const float *x = &p[u / 2][(u % 2) * 8];
                 pw[u] = make_uint4(Half16<DT>::pack(x[0], x[1]), Half16<DT>::pack(x[2], x[3]), Half16<DT>::pack(x[4], x[5]), Half16<DT>::pack(x[6], x[7]));
             }
         }
@@ -450,73 +469,77 @@ __global__ __launch_bounds__(kPromptThreads, PromptShape<DT>::kPerCu) void promp
     // O^T += V^T P.  2-byte types: a transposing read gives a lane four keys of its dim; two of them are the
     // eight keys 16u + 4kg + {0..3, 8..11} whose weights the lane holds in pw[u].
     auto value_product = [&](uint32_t vl, const uint4 (&pw)[kSteps]) {
-        int ln = lane;
-        asm volatile("" : "+v"(ln));
-        const int vkey = 4 * (ln >> 5) + ((ln & 15) >> 2), vpiece = ((ln >> 4) & 1) * 2 + ((ln & 3) >> 1);
-        const uint32_t at = vl + (kF32 ? (uint32_t)((ln >> 5) * 4 * kRowBytes + (ln & 31) * 4)
-                                       : (uint32_t)(vkey * kRowBytes + (vpiece ^ ((vkey & 7) << 1)) * 16 + (ln & 1) * 8));
+        if constexpr (kF32) {
 #pragma unroll
-        for (int u = 0; u < kSteps; ++u)
+            for (int u = 0; u < kSteps; ++u)
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt) {
-                if constexpr (kF32) {
-                    const float v = *(const lds_float *)(size_t)(at + (8 * (u / 4) + u % 4) * kRowBytes + dt * 128);
+                for (int dt = 0; dt < 4; ++dt) {
+                    const float v = *reinterpret_cast<const float *>(lds + (vl - lds0) + (8 * (u / 4) + 4 * kg + u % 4) * kRowBytes + (dt * 32 + n) * 4);
                     acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, __uint_as_float(pw[u].x), acc[dt], 0, 0, 0);
-                } else {
-                    const uint32_t p = (at ^ (dt * 64)) + u * 16 * kRowBytes;
-                    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v *)(size_t)p));
-                    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v *)(size_t)(p + 8 * kRowBytes)));
-                    acc[dt] = Half16<DT>::mfma32(make_uint4(x.x, x.y, y.x, y.y), pw[u], acc[dt]);
                 }
-            }
+        } else {
+            const int i = lane & 15, key = 4 * kg + (i >> 2);
+            const int piece = ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
+#pragma unroll
+            for (int u = 0; u < kSteps; ++u)
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt) {
+                    const uint32_t at = vl + key * kRowBytes + (((dt * 4 + piece) ^ ((key & 7) << 1)) * 16) + (i & 1) * 8 + u * 16 * kRowBytes;
+                    const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v *)(size_t)at);
+                    const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v *)(size_t)(at + 8 * kRowBytes));
+                    const uint2 xw = __builtin_bit_cast(uint2, x), yw = __builtin_bit_cast(uint2, y);
+                    acc[dt] = Half16<DT>::mfma32(make_uint4(xw.x, xw.y, yw.x, yw.y), pw[u], acc[dt]);
+                }
+        }
     };
 
-    // The pipeline: tile x is computed, tile x + stages - 1 requested, the rows of the one behind it turned into
-    // addresses, the blocks of two more looked up; a barrier per tile.  The overlap of matrix products,
-    // softmax and LDS reads is between the workgroups that share the compute unit.
+    // The pipeline.  While tile x's weights and value product are computed, the scores of tile x + 1 are; K of
+    // tile x + stages and V of the one before it are requested, the blocks of tile x + 2 * stages looked up
+    // and those of x + stages + 1 turned into addresses.  What an iteration requests has arrived stages - 2
+    // iterations later.
     constexpr int kInFlight = (kStages - 2) * 2 * kLoads;
-    constexpr int kAhead = kStages - 1;                  // tiles between a fetch and its use
-    if (tid == 0) { poison[0] = 0; poison[1] = 0; }
+    if (tid == 0) poison[0] = 0;
     int t = next(t_begin), reach = t;
+    f32x16 s[kTT];
     if (t < t_end) {
-        __syncthreads();
-        for (int x = 0, at = t; x < kAhead + 3; ++x) {   // the first slots, in turn by the waves
-            if (x % kPromptWaves == wave) look_up(x, at);
-            reach = at;
-            at = next(at + 1);
-        }
+        for (int x = 0; x < wave; ++x) reach = next(reach + 1);
+        look_up(wave, reach);                            // (as many waves as slots)
         direct_loads_done<0>();
+        resolve(wave, reach);
         __syncthreads();
-        for (int x = wave; x <= kAhead; x += kPromptWaves) resolve(x, tile_at(x));
-        __syncthreads();
+        if (docs && wave == 0) reach = tile_at(kSlots - 1);
+        fetch_keys(0);
+        fetch_values(0);
 #pragma unroll
-        for (int x = 0; x < kAhead; ++x) fetch_tile(x, x);
+        for (int x = 1; x < kStages - 1; ++x) { fetch_keys(x); fetch_values(x); }
         direct_loads_done<kInFlight>();
         __syncthreads();
-        if (!all_see(t, wg_lo, wg_hi)) set_aside(lds + kVat);
+        if (!all_see(t, wg_whole)) set_aside(lds + kVat);
     }
-    int stage = 0;
 #pragma unroll 1
     for (int x = 0; t < t_end; ++x) {
-        const bool holes = __builtin_amdgcn_readfirstlane(poison[1]);
-        fetch_tile(x + kAhead, stage == 0 ? kAhead : stage - 1);
-        if (docs) reach = next(reach + 1);
-        if (wave == (x & 3)) look_up(x + kAhead + 3, docs ? reach : min(t_begin + x + kAhead + 3, t_end));
-        if (wave == ((x + 2) & 3)) resolve(x + kAhead + 1, tile_at(x + kAhead + 1));
-        f32x16 s;
+        const int t1 = tile_at(x + 1);
+        const char *kl = lds + (x & (kStages - 1)) * kTileBytes;
+        char *vl = lds + kVat + (x & (kStages - 1)) * kTileBytes;
         uint4 pw[kSteps];
-        score_product(lds0 + stage * kTileBytes, s);
-        finish_scores(s, t, x & (kSlots - 1), holes);
+        fetch_keys(x + kStages - 1);
+        fetch_values(x + kStages - 1);
+        score_product(kl, s);
+        finish_scores(s, t, x & (kSlots - 1));
         raise_maximum(largest(s));
         weigh(s, pw);
-        value_product(lds0 + kVat + stage * kTileBytes, pw);
-        t = tile_at(x + 1);
-        stage = stage + 1 == kStages ? 0 : stage + 1;
-        if (t < t_end) {
+        value_product(lds0 + (uint32_t)(vl - lds), pw);
+        if (wave == 0) {
+            if (x + kStages >= kSlots) resolve(x + kStages, tile_at(x + kStages));
+            if (docs) reach = next(reach + 1);
+            look_up(x + kSlots, docs ? reach : min(t_begin + x + kSlots, t_end));
+        }
+        if (t1 < t_end) {
             direct_loads_done<kInFlight>();
             __syncthreads();
-            if (!all_see(t, wg_lo, wg_hi)) set_aside(lds + kVat + stage * kTileBytes);
+            if (!all_see(t1, wg_whole)) set_aside(lds + kVat + ((x + 1) & (kStages - 1)) * kTileBytes);
         }
+        t = t1;
     }
     direct_loads_done<0>();                              // (no load may reach the LDS after the workgroup has left it)
     l += __shfl_xor(l, 32, kWave);
@@ -524,7 +547,7 @@ __global__ __launch_bounds__(kPromptThreads, PromptShape<DT>::kPerCu) void promp
 #pragma unroll 1
         for (t = next(t_begin); t < t_end; t = next(t + 1)) {
             const int k0 = key_tile(t);
-            if (all_see(t, wg_lo, wg_hi)) continue;
+            if (all_see(t, wg_whole)) continue;
 #pragma unroll 1
             for (int j = k0; j < min(k0 + KT, len); ++j) {
                 const int64_t off = checked_row_bytes(a.kv, a.blocks, b, h, j);
@@ -574,23 +597,55 @@ __global__ __launch_bounds__(kPromptThreads, PromptShape<DT>::kPerCu) void promp
 
 // ---- weight of every key, summed over the last rows of the prompts -----------------------------
 // With every row's log-sum-exp known the weights are one product K Q^T and an exp2 away.  A wave keeps 32
-// keys as the first operand in registers and walks the counted rows; every lane sums its rows' weights
-// of 16 keys, the lanes are summed at the end: no atomics, one owner per key.
+// keys as the first operand in registers; the counted rows pass by in tiles of 32, which the four waves of
+// a workgroup share in LDS (a row's pieces lie 256 bytes apart for the lanes of an operand: read from
+// memory by every wave they took four times the requests).  Every lane sums its rows' weights of 16
+// keys, the lanes are summed at the end: no atomics, one owner per key.
+constexpr int kMassWaves = 4;
+
 template <int DT>
-__global__ __launch_bounds__(256, 2) void prompt_mass_kernel(PromptArgs a) {
+__global__ __launch_bounds__(kMassWaves * kWave, 2) void prompt_mass_kernel(PromptArgs a) {
     constexpr bool kF32 = DT == PQHSA_F32;
-    constexpr int kSlices = kD * (kF32 ? 4 : 2) / 32;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid / kWave;
+    constexpr int kRowBytes = kD * (kF32 ? 4 : 2), kSlices = kRowBytes / 32, kRowLanes = kRowBytes / 16, kPass = 64 / kRowLanes;
+    constexpr int kTile = 32 * kRowBytes, kLoads = kTile / 1024 / kMassWaves;
+    __shared__ __align__(16) char tiles[2 * kTile];
+    const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char *)tiles;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n = lane & 31, kg = lane >> 5;
     const int b = blockIdx.y / a.H, h = blockIdx.y - b * a.H;
-    const int len = sequence_length(a.seq_lens, b, a.n_max);
-    const int k0 = (blockIdx.x * 4 + wave) * 32;
-    if (k0 >= len) return;                               // (no barrier below: waves are independent)
-    const PromptRows rows = sequence_rows(a.cu_rows, a.T, b);
+    const int len = __builtin_amdgcn_readfirstlane(sequence_length(a.seq_lens, b, a.n_max));
+    const int wg_k0 = blockIdx.x * kMassWaves * 32, k0 = wg_k0 + wave * 32;
+    if (wg_k0 >= len) return;
+    const int wg_last = min(wg_k0 + kMassWaves * 32, len) - 1;
+    PromptRows rows = sequence_rows(a.cu_rows, a.T, b);
+    rows.first = __builtin_amdgcn_readfirstlane((int)rows.first);
+    rows.rows = __builtin_amdgcn_readfirstlane(rows.rows);
     const int first_pos = len - rows.rows;
-    const int prefix = min(sequence_prefix(a.score, b), len);
+    const int prefix = __builtin_amdgcn_readfirstlane(min(sequence_prefix(a.score, b), len));
     const int window = a.score.window > 0 ? a.score.window : 0x7fffffff;
     const int32_t *docs = a.score.docs ? a.score.docs + (int64_t)b * a.score.docs_stride : nullptr;
+
+    const int from = a.mass_rows > 0 ? max(0, rows.rows - a.mass_rows) : 0;
+    const int packed = rows.rows * a.G;
+    int at = from * a.G;
+    // rows before the first that can see a key of the workgroup (causal order, unless the prefix reaches one)
+    if (wg_k0 >= prefix) at = max(at, max(wg_k0 - first_pos, 0) * a.G);
+    const uint32_t magic = 0xffffffffu / (uint32_t)a.G;
+    auto token_of = [&](int pr) {                        // pr / G: the product is one short at most
+        const int t = (int)__umulhi((uint32_t)pr, magic);
+        return pr - t * a.G >= a.G ? t + 1 : t;
+    };
+    // rows at .. at + 31 into LDS (pieces placed as the prompt kernel's K); rows past the end repeat the last
+    auto fetch = [&](int at, int buf) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = (wave * kLoads + i) * kPass + lane / kRowLanes;
+            const int pr = min(at + r, packed - 1), token = token_of(pr);
+            const char *p = a.q + ((rows.first + token) * a.q_row + (int64_t)(h * a.G + pr - token * a.G) * a.q_head) * a.kv.esize;
+            load_direct(lds0 + buf * kTile + (wave * kLoads + i) * 1024, p + ((lane % kRowLanes) ^ (r & 15)) * 16);
+        }
+    };
+    if (at < packed) fetch(at, 0);
 
     uint4 kf[kSlices];
     const int64_t off = k0 + n < len ? checked_row_bytes(a.kv, a.blocks, b, h, k0 + n) : -1;
@@ -598,34 +653,27 @@ __global__ __launch_bounds__(256, 2) void prompt_mass_kernel(PromptArgs a) {
     for (int u = 0; u < kSlices; ++u)
         kf[u] = *reinterpret_cast<const uint4 *>(a.kv.k_base + (off < 0 ? 0 : off) + (u * 2 + kg) * 16);
     const uint32_t ok = (uint32_t)__ballot(off >= 0);    // (both halves of the wave hold the same 32 keys)
-    int kd[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int j = k0 + 8 * (r / 4) + 4 * kg + r % 4;
-        kd[r] = docs && j < len ? docs[j] : 0;
-    }
+    const bool general = a.score.capped || a.score.slopes || docs;
     float sum[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) sum[r] = 0.0f;
+    direct_loads_done<0>();
+    __syncthreads();
 
-    const int from = a.mass_rows > 0 ? max(0, rows.rows - a.mass_rows) : 0;
-    const int64_t packed = (int64_t)rows.rows * a.G;
-    int64_t at = (int64_t)from * a.G;
-    // rows before the first that can see a key of this tile (causal order, unless the prefix reaches it)
-    if (k0 >= prefix) at = max(at, (int64_t)max(k0 - first_pos, 0) * a.G);
-    for (; at < packed; at += 32) {
+    for (int buf = 0; at < packed; at += 32, buf ^= 1) {
+        // past the window of all the workgroup's keys, and these are not in the prefix: no later row sees them
+        const int first_row = first_pos + token_of(at);
+        if (wg_k0 >= prefix && first_row - wg_last >= window) break;
+        if (at + 32 < packed) fetch(at + 32, buf ^ 1);
         const bool mine = at + n < packed;
-        const int prc = (int)(mine ? at + n : packed - 1);
-        const int token = prc / a.G, g = prc - token * a.G, pos = first_pos + token;
-        // past the window of all the tile's keys, and these are not in the prefix: no later row sees them
-        if (k0 >= prefix && first_pos + (int)(at / a.G) - (k0 + 31) >= window) break;
-        const char *p = a.q + ((rows.first + token) * a.q_row + (int64_t)(h * a.G + g) * a.q_head) * a.kv.esize;
+        const int pr = min(at + n, packed - 1), token = token_of(pr), g = pr - token * a.G, pos = first_pos + token;
+        const float lse = a.lse[(rows.first + token) * (int64_t)(a.H * a.G) + h * a.G + g];
         f32x16 s;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.0f;
 #pragma unroll
         for (int u = 0; u < kSlices; ++u) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(p + (u * 2 + kg) * 16);
+            const uint4 x = *reinterpret_cast<const uint4 *>(tiles + buf * kTile + n * kRowBytes + (((u * 2 + kg) ^ (n & 15)) * 16));
             if constexpr (kF32) {
                 const f32x4 y = __builtin_bit_cast(f32x4, kf[u]), z = __builtin_bit_cast(f32x4, x);
 #pragma unroll
@@ -634,20 +682,29 @@ __global__ __launch_bounds__(256, 2) void prompt_mass_kernel(PromptArgs a) {
                 s = Half16<DT>::mfma32(kf[u], x, s);
             }
         }
-        const float lse = a.lse[(rows.first + token) * (int64_t)(a.H * a.G) + h * a.G + g];
         const float total = !mine || lse == -INFINITY ? INFINITY : lse * kLog2e;   // +inf: the row gives no weight
-        const float slope2 = a.score.slopes ? a.score.slopes[h * a.G + g] * kLog2e : 0.0f;
-        const int row_doc = docs && pos >= 0 ? docs[pos] : 0;
-        const int row_prefix = pos >= 0 ? prefix : 0, row_from = pos >= 0 ? max(pos - window + 1, 0) : 0;
+        const int last_row = first_pos + token_of(min(at + 31, packed - 1));
+        if (!general && ok == ~0u && first_row >= k0 + 31 && last_row - k0 < window) {   // every row sees every key
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int jj = 8 * (r / 4) + 4 * kg + r % 4, j = k0 + jj;
-            float z = a.score.capped ? a.score.cap2 * tanh_score(s[r] * a.score.in_cap) : s[r] * a.score.scale2;
-            z -= slope2 * (float)abs(pos - j);
-            const bool see = ((j >= row_from && j <= pos) || j < row_prefix) && ((ok >> jj) & 1) && (!docs || kd[r] == row_doc);
-            sum[r] += see && mine ? exp2_fast(z - total) : 0.0f;
+            for (int r = 0; r < 16; ++r) sum[r] += exp2_fast(__builtin_fmaf(s[r], a.score.scale2, -total));
+        } else {
+            const float slope2 = a.score.slopes ? a.score.slopes[h * a.G + g] * kLog2e : 0.0f;
+            const int row_doc = docs && pos >= 0 ? docs[pos] : 0;
+            const int row_prefix = pos >= 0 ? prefix : 0, row_from = pos >= 0 ? max(pos - window + 1, 0) : 0x7fffffff;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int jj = 8 * (r / 4) + 4 * kg + r % 4, j = k0 + jj;
+                float z = a.score.capped ? a.score.cap2 * tanh_score(s[r] * a.score.in_cap) : s[r] * a.score.scale2;
+                z -= slope2 * (float)abs(pos - j);
+                uint32_t see = (((j >= row_from) & (j <= pos)) | (j < row_prefix)) & (ok >> jj);
+                if (docs) see &= j < len && docs[j] == row_doc;
+                sum[r] += see & 1 ? exp2_fast(z - total) : 0.0f;
+            }
         }
+        direct_loads_done<0>();
+        __syncthreads();
     }
+    direct_loads_done<0>();
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         float x = sum[r];
@@ -667,23 +724,30 @@ __global__ __launch_bounds__(256, 2) void prompt_mass_kernel(PromptArgs a) {
 namespace {
 
 struct PromptPlan {
+    int waves;
     int64_t tiles;
     int splits;
     size_t ml_at, lse_at, bytes;
 };
 
-PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint, bool own_lse) {
+PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint, int key_tile, bool own_lse) {
     PromptPlan p = {};
-    p.tiles = (T * G + kPromptRows - 1) / kPromptRows + B;              // every sequence may end inside a tile
+    // Eight waves (256 rows, four stages, one workgroup per compute unit) halve the K/V traffic of four (128
+    // rows, two stages, two workgroups), which overlap each other's starts and ends.
+    p.waves = T * G / 256 * H >= 512 ? 8 : 4;
+    const int tile_rows = p.waves * 32;
+    p.tiles = (T * G + tile_rows - 1) / tile_rows + B;              // every sequence may end inside a tile
     int64_t busy = p.tiles - B;
     if (rows_hint > 0 && rows_hint * (int64_t)B <= T) {             // about as many tiles as sequences have
-        const int64_t each = ((int64_t)rows_hint * G + kPromptRows - 1) / kPromptRows;
+        const int64_t each = ((int64_t)rows_hint * G + tile_rows - 1) / tile_rows;
         if (each * B > busy) busy = each * B;
     }
     if (busy < 1) busy = 1;
-    // fill the chip, with at least four key tiles a workgroup
-    const int64_t want = (kPromptFill + busy * H - 1) / (busy * H);
-    const int64_t most = ((int64_t)n_max + 255) / 256;
+    // fill the chip with keys enough a workgroup to be worth the join (a launch and the partial sums' way
+    // through memory, 8 us: eight tiles of the 2-byte types, two of fp32 take that long)
+    const int64_t want = ((p.waves == 8 ? 256 : 512) + busy * H - 1) / (busy * H);
+    const int64_t least = key_tile == 32 ? 64 : 512;
+    const int64_t most = ((int64_t)n_max + least - 1) / least;
     p.splits = (int)(want < most ? want : most);
     if (p.splits < 1) p.splits = 1;
     const size_t rows = (size_t)T * H * G;
@@ -698,16 +762,16 @@ PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint,
     return p;
 }
 
-template <int DT, bool GENERAL>
+template <int DT, bool GENERAL, int WAVES>
 int launch_prompt(const PromptArgs &a, hipStream_t stream) {
-    auto kern = prompt_attend_kernel<DT, GENERAL>;
-    const size_t lds = PromptShape<DT>::kLds + 2 * (size_t)a.mask_words * 4;
+    auto kern = prompt_attend_kernel<DT, GENERAL, WAVES>;
+    const size_t lds = PromptShape<WAVES>::kLds + 2 * (size_t)a.mask_words * 4;
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) {
         set_error("prompt_attend: cannot raise the LDS limit to %zu: %s", lds, hipGetErrorString(e));
         return PQHSA_ELAUNCH;
     }
-    hipLaunchKernelGGL(kern, dim3((unsigned)(a.H * a.tiles * a.splits)), dim3(kPromptThreads), lds, stream, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.H * a.tiles * a.splits)), dim3(WAVES * kWave), lds, stream, a);
     return check_launch("prompt_attend");
 }
 
@@ -720,7 +784,7 @@ using namespace pqhsa;
 extern "C" size_t pqhsa_prompt_attend_workspace_bytes(int64_t T, int32_t B, int32_t H, int32_t G, int32_t n_max,
                                                       int32_t rows_hint, int32_t dtype, int32_t with_lse) {
     if (T <= 0 || B <= 0 || H <= 0 || G <= 0 || n_max <= 0) return 256;
-    const size_t need = plan_prompt(T, B, H, G, n_max, rows_hint, with_lse == 0).bytes;
+    const size_t need = plan_prompt(T, B, H, G, n_max, rows_hint, dtype == PQHSA_F32 ? 32 : 64, with_lse == 0).bytes;
     return need < 256 ? 256 : need;
 }
 
@@ -753,7 +817,8 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
                       "%s: %d blocks, and a table of %d x %d tokens for n_max %d", what, blocks, kv->max_blocks, kv->block_size, n_max);
     PQHSA_REQUIRE(T * G < 0x7fffffff && T * H * G < 0x7fffffff, "%s: %lld rows of %d x %d heads are too many", what, (long long)T, H, G);
     PQHSA_REQUIRE((int64_t)B * H <= 65535, "%s: too many sequences and heads", what);
-        const PromptPlan p = plan_prompt(T, B, H, G, n_max, rows_hint, lse == nullptr);
+    const int key_tile = kv->dtype == PQHSA_F32 ? 32 : 64;
+    const PromptPlan p = plan_prompt(T, B, H, G, n_max, rows_hint, key_tile, lse == nullptr);
     PQHSA_REQUIRE(p.tiles * H * p.splits <= 0x7fffffff, "%s: %lld row tiles are too many for one launch", what, (long long)p.tiles);
     if (workspace_bytes < p.bytes) {
         set_error("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, p.bytes);
@@ -771,14 +836,15 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
     a.tiles = (int)p.tiles;
     a.block_magic = kv->paged ? 0xffffffffu / (uint32_t)kv->block_size : 0u;
     a.splits = p.splits;
-    a.mask_words = score->docs ? (n_max / KT + 2 + 31) / 32 + 1 : 0;
+    a.mask_words = score->docs ? (n_max / key_tile + 2 + 31) / 32 + 1 : 0;
     a.part_o = reinterpret_cast<float *>(w);
     a.part_ml = reinterpret_cast<float2 *>(w + p.ml_at);
-    const size_t most_lds = PromptShape<PQHSA_F32>::kLds + 2 * (size_t)a.mask_words * 4;
-    PQHSA_REQUIRE(most_lds <= 160 * 1024, "%s: n_max %d too large for a document mask", what, n_max);
+    PQHSA_REQUIRE(PromptShape<8>::kLds + 2 * (size_t)a.mask_words * 4 <= 160 * 1024, "%s: n_max %d too large for a document mask", what, n_max);
     if (T > 0) {
         const bool general = score->softcap > 0.0f || score->slopes || !(score->scale > 0.0f);
-        PQHSA_DISPATCH_DTYPE(kv->dtype, rc = general ? launch_prompt<DT, true>(a, stream) : launch_prompt<DT, false>(a, stream));
+        PQHSA_DISPATCH_DTYPE(kv->dtype, 
+                              if (p.waves == 8) rc = general ? launch_prompt<DT, true, 8>(a, stream) : launch_prompt<DT, false, 8>(a, stream);
+                              else rc = general ? launch_prompt<DT, true, 4>(a, stream) : launch_prompt<DT, false, 4>(a, stream));
         if (rc) return rc;
         if (p.splits > 1) {
             JoinArgs j = {a.part_o, a.part_ml, p.splits, H * G, a.out, a.out_row, a.out_head, a.lse, cu_rows + B};
@@ -788,8 +854,9 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
     }
     if (mass && n_max > 0) {
         a.mass_in = mass->in; a.mass_out = mass->out; a.mass_stride = mass->stride; a.decay = mass->decay; a.mass_rows = mass->rows;
-        const dim3 grid((unsigned)((n_max + 127) / 128), (unsigned)(B * H));
-        PQHSA_DISPATCH_DTYPE(kv->dtype, hipLaunchKernelGGL(prompt_mass_kernel<DT>, grid, dim3(256), 0, stream, a));
+        const int keys = kMassWaves * 32;
+        const dim3 grid((unsigned)((n_max + keys - 1) / keys), (unsigned)(B * H));
+        PQHSA_DISPATCH_DTYPE(kv->dtype, hipLaunchKernelGGL(prompt_mass_kernel<DT>, grid, dim3(kMassWaves * kWave), 0, stream, a));
         rc = check_launch("prompt_mass");
     }
     return rc;
