@@ -405,6 +405,7 @@ int64_t visible_bound(const pqhsa_score *s, int64_t n_max) {
 
 int validate_score(const pqhsa_score *s, int n_max, const char *what) {
     PQHSA_REQUIRE(s != nullptr, "%s: score rule is NULL", what);
+    PQHSA_REQUIRE(n_max <= 0x7fffffff - 65536, "%s: n_max %d is too large (key numbers are 32 bits)", what, n_max);
     PQHSA_REQUIRE(isfinite(s->scale), "%s: scale is not finite", what);
     PQHSA_REQUIRE(isfinite(s->softcap) && s->softcap >= 0.0f, "%s: softcap must be finite and not negative", what);
     PQHSA_REQUIRE(s->window >= 0 && s->prefix >= 0, "%s: window %d and prefix %d must not be negative", what, s->window, s->prefix);

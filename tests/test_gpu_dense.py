@@ -202,6 +202,7 @@ def test_rule_refusals_without_a_gpu():
             ops.ScoreRule(**kw)
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: a call that were not refused must find no GPU")
 def test_c_entry_refuses_bad_arguments_before_any_gpu_work():
     import ctypes
 
@@ -219,6 +220,7 @@ def test_c_entry_refuses_bad_arguments_before_any_gpu_work():
     assert call(q=None) == -1 and call(q=(1 << 20) + 8) == -1 and call(stride=4) == -1
     assert call(dtype=_lib.F32) == -1 and b"dtype" in lib.pqhsa_last_error()
     assert call(n_max=-1) == -1 and call(ws=(1 << 20) + 16) == -1
+    assert call(n_max=2**31 - 1, ws_bytes=1 << 60) == -1 and b"large" in lib.pqhsa_last_error()
     assert call(n_max=1 << 20, ws_bytes=16) == -3 and b"workspace" in lib.pqhsa_last_error()
     mass.decay = 1.0
     assert call(mass=ctypes.byref(mass)) == -1
