@@ -493,21 +493,21 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
         }
     };
 
-    // The pipeline.  While tile x's weights and value product are computed, the scores of tile x + 1 are; K of
-    // tile x + stages and V of the one before it are requested, the blocks of tile x + 2 * stages looked up
-    // and those of x + stages + 1 turned into addresses.  What an iteration requests has arrived stages - 2
-    // iterations later.
+    // The ring.  While tile x is computed, K and V of tile x + stages - 1 are requested, the blocks of tile
+    // x + slots - 1 looked up and those of tile x + stages turned into addresses.  What iteration x requests has
+    // arrived by the end of iteration x + stages - 2.  Tile x's own slot is still being read (its documents),
+    // so the first that may be looked up anew is the one of tile x - 1.
     constexpr int kInFlight = (kStages - 2) * 2 * kLoads;
     if (tid == 0) poison[0] = 0;
     int t = next(t_begin), reach = t;
     f32x16 s[kTT];
     if (t < t_end) {
         for (int x = 0; x < wave; ++x) reach = next(reach + 1);
-        look_up(wave, reach);                            // (as many waves as slots)
+        if (wave < kSlots - 1) look_up(wave, reach);     // (as many waves as slots; the last slot is iteration 0's)
         direct_loads_done<0>();
-        resolve(wave, reach);
+        if (wave < kSlots - 1) resolve(wave, reach);
         __syncthreads();
-        if (docs && wave == 0) reach = tile_at(kSlots - 1);
+        if (docs && wave == 0) reach = tile_at(kSlots - 2);
         fetch_keys(0);
         fetch_values(0);
 #pragma unroll
@@ -530,9 +530,9 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
         weigh(s, pw);
         value_product(lds0 + (uint32_t)(vl - lds), pw);
         if (wave == 0) {
-            if (x + kStages >= kSlots) resolve(x + kStages, tile_at(x + kStages));
+            if (x + kStages >= kSlots - 1) resolve(x + kStages, tile_at(x + kStages));
             if (docs) reach = next(reach + 1);
-            look_up(x + kSlots, docs ? reach : min(t_begin + x + kSlots, t_end));
+            look_up(x + kSlots - 1, docs ? reach : min(t_begin + x + kSlots - 1, t_end));
         }
         if (t1 < t_end) {
             direct_loads_done<kInFlight>();

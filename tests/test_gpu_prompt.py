@@ -161,6 +161,27 @@ def test_block_table_entries_outside_the_cache_mask_their_keys():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_documents_that_alternate_between_keys_over_many_tiles(dtype):
+    """Every tile of the walk is masked by its own keys' documents, which are read while later tiles' are on their way."""
+    p = PromptProblem([1500, 900], [1500, 500], heads=1, groups=4, dtype=dtype, seed=41, docs=3)
+    p.docs = torch.randint(0, 3, p.docs.shape, generator=torch.Generator().manual_seed(5)).to(torch.int32)
+    check(p, mass=0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("kw", [dict(), dict(docs=3), dict(window=300, prefix=20, softcap=30.0)])
+def test_rows_enough_for_the_large_workgroups(dtype, kw):
+    """131072 packed rows and more: eight waves a workgroup, four tiles of K and V in LDS."""
+    p = PromptProblem([901, 700, 512, 900, 650, 640, 577, 830], [512, 500, 512, 550, 520, 515, 490, 500], heads=2, groups=16,
+                      dtype=dtype, seed=43, **kw)
+    if "docs" in kw:
+        p.docs = torch.randint(0, 3, p.docs.shape, generator=torch.Generator().manual_seed(5)).to(torch.int32)
+    check(p, mass=3)
+
+
+@gpu
 def test_same_results_without_lse_and_from_a_replayed_graph():
     p = PromptProblem([260, 90], [260, 40], heads=2, groups=4, seed=31)
     kv, rule, q, sl, cu = p.source(), p.rule(), p.q.cuda(), p.seq_lens(), p.cu_rows()
@@ -211,6 +232,7 @@ def test_refusals():
     refused("prefix", rule=ops.ScoreRule(scale=SCALE, prefix=torch.zeros(3, dtype=torch.int32, device="cuda")))
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: a call that were not refused must find no GPU")
 def test_c_entry_refuses_bad_arguments_before_any_gpu_work():
     import ctypes
 
@@ -227,8 +249,9 @@ def test_c_entry_refuses_bad_arguments_before_any_gpu_work():
     assert call(G=17) == -1 and b"16" in lib.pqhsa_last_error()
     assert call(q=None) == -1 and call(q=(1 << 20) + 8) == -1 and call(stride=4) == -1
     assert call(dtype=_lib.F32) == -1 and call(n_max=-1) == -1 and call(T=-1) == -1 and call(ws=(1 << 20) + 16) == -1
+    assert call(n_max=2**31 - 1, ws_bytes=1 << 60) == -1 and b"large" in lib.pqhsa_last_error()
     assert call(n_max=1 << 20, ws_bytes=16) == -3 and b"workspace" in lib.pqhsa_last_error()
-    assert call(T=1 << 30, H=4) == -1 and call(T=1 << 24, H=1, ws_bytes=1 << 60) == -1     # more than one launch holds
+    assert call(T=1 << 30, H=4) == -1                              # more rows than one launch numbers
     assert call(B=70000, H=1) == -1
     mass.out, mass.stride, mass.decay, mass.rows = 1 << 20, 10, 1.0, -1
     assert call(mass=ctypes.byref(mass)) == -1
