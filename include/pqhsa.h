@@ -505,11 +505,11 @@ int pqhsa_dense_attend_paged(const void *q, int32_t q_dtype, int64_t q_stride_ro
  * cache's dtype; rows of out and lse past cu_rows[B] are left as they are.  A row in front of its
  * sequence (more rows than tokens) sees nothing.  lse f32 [T, H * G], mass: may be NULL.  rows_hint:
  * the largest number of rows of a sequence, 0 = unknown (sizes the launch, results do not depend on
- * it beyond summation order).  n_max, blocks, workspace: as above; `with_lse` is 0 when lse is NULL.
- * B * H <= 65535, T * H * G < 2^31, at most 65535 * 128 packed rows (T * G).
+ * it beyond summation order).  n_max, blocks, workspace: as above; `with_mass` is 0 when mass is NULL.
+ * B * H <= 65535, T * H * G < 2^31; with docs, n_max up to about a million (a bit per key tile in LDS).
  */
 size_t pqhsa_prompt_attend_workspace_bytes(int64_t T, int32_t B, int32_t H, int32_t G, int32_t n_max,
-                                           int32_t rows_hint, int32_t dtype, int32_t with_lse);
+                                           int32_t rows_hint, int32_t dtype, int32_t with_mass);
 int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t q_stride_row, int64_t q_stride_head,
                               void *out, int64_t out_stride_row, int64_t out_stride_head, int64_t T,
                               const int32_t *cu_rows, const pqhsa_kv_view *kv, int32_t blocks, int32_t B,

@@ -291,50 +291,73 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_attend_kernel(DenseArg
 }
 
 // ---- join of the split partials: one workgroup per row -------------------------------------
-// The row's maximum and sum from all (m, l), then eight splits at a time, four dims a lane.
+// Eight groups of 32 lanes (four dims a lane) take every eighth split, eight of them at a time with all
+// loads in flight at once: few rows join, so the time is one or two round trips to memory.  Each group
+// keeps a running maximum and sum; the groups meet in LDS.
 template <int DT>
 __global__ __launch_bounds__(256) void dense_join_kernel(JoinArgs a) {
-    __shared__ float red[8][kD];
-    __shared__ float wm[4], wl[4];
+    constexpr int kGroups = 8, kBatch = 8;
+    __shared__ float red[kGroups][kD];
+    __shared__ float2 red_ml[kGroups];
     const int64_t r = blockIdx.x;
     const int64_t token = r / a.heads;
     if (a.row_count && token >= *a.row_count) return;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, group = tid / 32, d4 = tid % 32;
     const float2 *ml = a.part_ml + r * a.splits;
+    const float *part = a.part_o + r * a.splits * kD + d4 * 4;
     float m = -INFINITY, l = 0.0f;
-    for (int s = tid; s < a.splits; s += 256) {
-        const float2 x = ml[s];
-        const float to = fmaxf(m, x.x);
-        l = (m == to ? l : l * exp2_fast(m - to)) + (x.x == to ? x.y : x.y * exp2_fast(x.x - to));
-        m = to;
-    }
-    const float wtop = wave_max_all(m);
-    l = wave_total(m == wtop ? l : l * exp2_fast(m - wtop));
-    if ((tid & 63) == 0) { wm[tid / 64] = wtop; wl[tid / 64] = l; }
-    __syncthreads();
-    m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-    l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) l += wm[w] == m ? wl[w] : wl[w] * exp2_fast(wm[w] - m);
-    const int sl = tid / 32, d4 = tid % 32;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int s = sl; s < a.splits; s += 8) {
-        const float ms = ml[s].x;
-        if (ms == -INFINITY) continue;                   // a split without a visible key wrote no sums
-        const float f = ms == m ? 1.0f : exp2_fast(ms - m);
-        const float4 x = *reinterpret_cast<const float4 *>(a.part_o + (r * a.splits + s) * kD + d4 * 4);
-        o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
+    for (int s0 = group; s0 < a.splits; s0 += kGroups * kBatch) {
+        float2 y[kBatch];
+        float4 x[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int s = min(s0 + i * kGroups, a.splits - 1);
+            y[i] = ml[s];
+            x[i] = *reinterpret_cast<const float4 *>(part + (int64_t)s * kD);
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (s0 + i * kGroups >= a.splits) y[i] = make_float2(-INFINITY, 0.0f);
+            top = fmaxf(top, y[i].x);
+        }
+        const float back = m == top ? 1.0f : exp2_fast(m - top);
+        m = top;
+        l *= back;
+        o.x *= back; o.y *= back; o.z *= back; o.w *= back;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            // a split without a visible key wrote no sums: whatever lies there is not used
+            const bool some = y[i].y != 0.0f;            // (NaN counts)
+            const float f = y[i].x == m ? 1.0f : exp2_fast(y[i].x - m);
+            l += some ? f * y[i].y : 0.0f;
+            o.x += some ? f * x[i].x : 0.0f;
+            o.y += some ? f * x[i].y : 0.0f;
+            o.z += some ? f * x[i].z : 0.0f;
+            o.w += some ? f * x[i].w : 0.0f;
+        }
     }
-    *reinterpret_cast<float4 *>(&red[sl][d4 * 4]) = o;
+    *reinterpret_cast<float4 *>(&red[group][d4 * 4]) = o;
+    if (d4 == 0) red_ml[group] = make_float2(m, l);
     __syncthreads();
     if (tid < kD) {
-        float x = 0.0f;
+        float2 y[kGroups];
+        m = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) x += red[w][tid];
+        for (int w = 0; w < kGroups; ++w) { y[w] = red_ml[w]; m = fmaxf(m, y[w].x); }
+        float x = 0.0f;
+        l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kGroups; ++w) {
+            const float f = y[w].x == m ? 1.0f : exp2_fast(y[w].x - m);   // (a group without a visible key holds zeros)
+            l += f * y[w].y;
+            x += f * red[w][tid];
+        }
         constexpr int esize = DT == PQHSA_F32 ? 4 : 2;
         store1<DT>(a.out + (token * a.out_row + (r - token * a.heads) * a.out_head) * esize, tid, l == 0.0f ? 0.0f : x / l);
         if (tid == 0 && a.lse) a.lse[r] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+        if (tid == 0 && a.row_ml) a.row_ml[r] = make_float2(m, l);
     }
 }
 
@@ -362,7 +385,7 @@ struct MassArgs {
 };
 
 __global__ __launch_bounds__(256) void dense_mass_kernel(MassArgs a) {
-    __shared__ float total[kDenseRows];                  // log2 sum of every row
+    __shared__ float2 row[kDenseRows];                   // maximum and 1 / sum of every row
     const int bh = blockIdx.y, b = bh / a.H;
     const int len = sequence_length(a.seq_lens, b, a.n_max);
     const int j0 = blockIdx.x * kMassKeys;
@@ -380,7 +403,7 @@ __global__ __launch_bounds__(256) void dense_mass_kernel(MassArgs a) {
         }
         const float top = wave_max_all(m);
         l = wave_total(m == top ? l : l * exp2_fast(m - top));
-        if (lane == 0) total[g] = l == 0.0f ? INFINITY : top + log2f(l);   // +inf: the row gives no weight
+        if (lane == 0) row[g] = l == 0.0f ? make_float2(INFINITY, 0.0f) : make_float2(top, 1.0f / l);   // +inf: the row gives no weight
     }
     __syncthreads();
     const float *scores = a.scores + (int64_t)bh * a.G * a.score_stride;
@@ -391,7 +414,7 @@ __global__ __launch_bounds__(256) void dense_mass_kernel(MassArgs a) {
         float w = a.in ? a.decay * a.in[(int64_t)bh * a.stride + j] : 0.0f;
         const int v = j < range.first ? j : j - range.gap;
         if (j < range.first || v >= range.first)
-            for (int g = 0; g < a.G; ++g) w += exp2_fast(scores[g * a.score_stride + v] - total[g]);
+            for (int g = 0; g < a.G; ++g) w = __builtin_fmaf(exp2_fast(scores[g * a.score_stride + v] - row[g].x), row[g].y, w);
         a.out[(int64_t)bh * a.stride + j] = w;
     }
 }
@@ -434,8 +457,11 @@ DensePlan plan_dense(int B, int H, int G, int n_max, const pqhsa_score *score, b
     DensePlan p = {};
     const int64_t streams = (int64_t)B * H;
     const int64_t keys = visible_bound(score, n_max) > 0 ? visible_bound(score, n_max) : 1;
-    // about 1024 workgroups, two rounds of what the chip holds at once
-    int64_t chunk = (streams * keys + 1023) / 1024;
+    // The chip holds 512 workgroups at once.  One sequence's chunks are equally long, so it is cut into one
+    // such round (1 x 32768: 30.8 us, 33.7 in three rounds); several are as long as the longest at most, and
+    // three rounds even that out (16 of 16384 to 65536 keys: 360 us, 381 in two).
+    const int64_t want = B == 1 ? 512 : 1536;
+    int64_t chunk = (streams * keys + want - 1) / want;
     chunk = (chunk + kDenseChunkMin - 1) / kDenseChunkMin * kDenseChunkMin;
     if (chunk > kDenseChunkMax) chunk = kDenseChunkMax;
     p.chunk = (int)chunk;
@@ -517,7 +543,7 @@ extern "C" int pqhsa_dense_attend_paged(const void *q, int32_t q_dtype, int64_t 
     rc = check_launch(what);
     if (rc) return rc;
     if (p.splits > 1) {
-        JoinArgs j = {a.part_o, a.part_ml, p.splits, H * G, a.out, a.out_row, a.out_head, lse, nullptr};
+        JoinArgs j = {a.part_o, a.part_ml, p.splits, H * G, a.out, a.out_row, a.out_head, lse, nullptr, nullptr};
         rc = launch_join(j, kv->dtype, (int64_t)B * H * G, stream);
         if (rc) return rc;
     }

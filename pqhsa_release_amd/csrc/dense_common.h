@@ -149,6 +149,7 @@ struct JoinArgs {
     char *out;
     int64_t out_row, out_head; // strides in elements
     float *lse;                // [rows, heads] or NULL
+    float2 *row_ml;            // [rows, heads] maximum and sum, or NULL
     const int32_t *row_count;  // rows in use (device), NULL: all
 };
 int launch_join(const JoinArgs &a, int dtype, int64_t rows, hipStream_t stream);

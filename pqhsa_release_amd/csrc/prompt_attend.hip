@@ -52,6 +52,7 @@ struct PromptArgs {
     int mask_words;                    // words of the per-tile bit mask in LDS (documents)
     float *part_o;                     // [T * H * G, splits, 128]
     float2 *part_ml;                   // [T * H * G, splits]
+    float2 *row_ml;                    // [T * H * G] maximum and sum of every row (accumulated weights only)
     // accumulated weights
     const float *mass_in;
     float *mass_out;
@@ -580,6 +581,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
         return;
     }
     if (kg == 0 && a.lse) a.lse[r] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    if (kg == 0 && a.row_ml) a.row_ml[r] = make_float2(m, l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     char *o = a.out + ((rows.first + token) * a.out_row + (int64_t)(h * a.G + g) * a.out_head) * a.kv.esize;
 #pragma unroll
@@ -596,7 +598,8 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
 }
 
 // ---- weight of every key, summed over the last rows of the prompts -----------------------------
-// With every row's log-sum-exp known the weights are one product K Q^T and an exp2 away.  A wave keeps 32
+// With every row's maximum m and sum l known the weights are one product K Q^T and an exp2 away (m and l
+// rather than the log-sum-exp: rounding that to fp32 would put 1e-6 of error on every weight).  A wave keeps 32
 // keys as the first operand in registers; the counted rows pass by in tiles of 32, which the four waves of
 // a workgroup share in LDS (a row's pieces lie 256 bytes apart for the lanes of an operand: read from
 // memory by every wave they took four times the requests).  Every lane sums its rows' weights of 16
@@ -667,7 +670,7 @@ __global__ __launch_bounds__(kMassWaves * kWave, 2) void prompt_mass_kernel(Prom
         if (at + 32 < packed) fetch(at + 32, buf ^ 1);
         const bool mine = at + n < packed;
         const int pr = min(at + n, packed - 1), token = token_of(pr), g = pr - token * a.G, pos = first_pos + token;
-        const float lse = a.lse[(rows.first + token) * (int64_t)(a.H * a.G) + h * a.G + g];
+        const float2 ml = a.row_ml[(rows.first + token) * (int64_t)(a.H * a.G) + h * a.G + g];
         f32x16 s;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.0f;
@@ -682,11 +685,12 @@ __global__ __launch_bounds__(kMassWaves * kWave, 2) void prompt_mass_kernel(Prom
                 s = Half16<DT>::mfma32(kf[u], x, s);
             }
         }
-        const float total = !mine || lse == -INFINITY ? INFINITY : lse * kLog2e;   // +inf: the row gives no weight
+        const bool gives = mine && ml.y != 0.0f;
+        const float m = gives ? ml.x : INFINITY, inv = gives ? 1.0f / ml.y : 0.0f;
         const int last_row = first_pos + token_of(min(at + 31, packed - 1));
         if (!general && ok == ~0u && first_row >= k0 + 31 && last_row - k0 < window) {   // every row sees every key
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum[r] += exp2_fast(__builtin_fmaf(s[r], a.score.scale2, -total));
+            for (int r = 0; r < 16; ++r) sum[r] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[r], a.score.scale2, -m)), inv, sum[r]);
         } else {
             const float slope2 = a.score.slopes ? a.score.slopes[h * a.G + g] * kLog2e : 0.0f;
             const int row_doc = docs && pos >= 0 ? docs[pos] : 0;
@@ -698,7 +702,7 @@ __global__ __launch_bounds__(kMassWaves * kWave, 2) void prompt_mass_kernel(Prom
                 z -= slope2 * (float)abs(pos - j);
                 uint32_t see = (((j >= row_from) & (j <= pos)) | (j < row_prefix)) & (ok >> jj);
                 if (docs) see &= j < len && docs[j] == row_doc;
-                sum[r] += see & 1 ? exp2_fast(z - total) : 0.0f;
+                sum[r] = __builtin_fmaf(see & 1 ? exp2_fast(z - m) : 0.0f, inv, sum[r]);
             }
         }
         direct_loads_done<0>();
@@ -727,10 +731,10 @@ struct PromptPlan {
     int waves;
     int64_t tiles;
     int splits;
-    size_t ml_at, lse_at, bytes;
+    size_t ml_at, row_at, bytes;
 };
 
-PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint, int key_tile, bool own_lse) {
+PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint, int key_tile, bool mass) {
     PromptPlan p = {};
     // Eight waves (256 rows, four stages, one workgroup per compute unit) halve the K/V traffic of four (128
     // rows, two stages, two workgroups), which overlap each other's starts and ends.
@@ -757,7 +761,7 @@ PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint,
         take(rows * p.splits * kD * sizeof(float));
         p.ml_at = take(rows * p.splits * sizeof(float2));
     }
-    if (own_lse) p.lse_at = take(rows * sizeof(float));
+    if (mass) p.row_at = take(rows * sizeof(float2));
     p.bytes = at;
     return p;
 }
@@ -782,9 +786,9 @@ int launch_prompt(const PromptArgs &a, hipStream_t stream) {
 using namespace pqhsa;
 
 extern "C" size_t pqhsa_prompt_attend_workspace_bytes(int64_t T, int32_t B, int32_t H, int32_t G, int32_t n_max,
-                                                      int32_t rows_hint, int32_t dtype, int32_t with_lse) {
+                                                      int32_t rows_hint, int32_t dtype, int32_t with_mass) {
     if (T <= 0 || B <= 0 || H <= 0 || G <= 0 || n_max <= 0) return 256;
-    const size_t need = plan_prompt(T, B, H, G, n_max, rows_hint, dtype == PQHSA_F32 ? 32 : 64, with_lse == 0).bytes;
+    const size_t need = plan_prompt(T, B, H, G, n_max, rows_hint, dtype == PQHSA_F32 ? 32 : 64, with_mass != 0).bytes;
     return need < 256 ? 256 : need;
 }
 
@@ -818,7 +822,7 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
     PQHSA_REQUIRE(T * G < 0x7fffffff && T * H * G < 0x7fffffff, "%s: %lld rows of %d x %d heads are too many", what, (long long)T, H, G);
     PQHSA_REQUIRE((int64_t)B * H <= 65535, "%s: too many sequences and heads", what);
     const int key_tile = kv->dtype == PQHSA_F32 ? 32 : 64;
-    const PromptPlan p = plan_prompt(T, B, H, G, n_max, rows_hint, key_tile, lse == nullptr);
+    const PromptPlan p = plan_prompt(T, B, H, G, n_max, rows_hint, key_tile, mass != nullptr);
     PQHSA_REQUIRE(p.tiles * H * p.splits <= 0x7fffffff, "%s: %lld row tiles are too many for one launch", what, (long long)p.tiles);
     if (workspace_bytes < p.bytes) {
         set_error("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, p.bytes);
@@ -829,7 +833,7 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
     PromptArgs a = {};
     a.q = static_cast<const char *>(q); a.q_row = q_stride_row; a.q_head = q_stride_head;
     a.out = static_cast<char *>(out); a.out_row = out_stride_row; a.out_head = out_stride_head;
-    a.lse = lse ? lse : reinterpret_cast<float *>(w + p.lse_at);
+    a.lse = lse;
     a.kv = make_view(kv);
     a.blocks = blocks; a.B = B; a.H = H; a.G = G; a.cu_rows = cu_rows; a.T = T; a.seq_lens = seq_lens; a.n_max = n_max;
     a.score = make_score(score);
@@ -839,6 +843,7 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
     a.mask_words = score->docs ? (n_max / key_tile + 2 + 31) / 32 + 1 : 0;
     a.part_o = reinterpret_cast<float *>(w);
     a.part_ml = reinterpret_cast<float2 *>(w + p.ml_at);
+    a.row_ml = mass ? reinterpret_cast<float2 *>(w + p.row_at) : nullptr;
     PQHSA_REQUIRE(PromptShape<8>::kLds + 2 * (size_t)a.mask_words * 4 <= 160 * 1024, "%s: n_max %d too large for a document mask", what, n_max);
     if (T > 0) {
         const bool general = score->softcap > 0.0f || score->slopes || !(score->scale > 0.0f);
@@ -847,7 +852,7 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
                               else rc = general ? launch_prompt<DT, true, 4>(a, stream) : launch_prompt<DT, false, 4>(a, stream));
         if (rc) return rc;
         if (p.splits > 1) {
-            JoinArgs j = {a.part_o, a.part_ml, p.splits, H * G, a.out, a.out_row, a.out_head, a.lse, cu_rows + B};
+            JoinArgs j = {a.part_o, a.part_ml, p.splits, H * G, a.out, a.out_row, a.out_head, a.lse, a.row_ml, cu_rows + B};
             rc = launch_join(j, kv->dtype, T * H * G, stream);
             if (rc) return rc;
         }

@@ -947,7 +947,7 @@ def prompt_attend(q: torch.Tensor, out: torch.Tensor, kv: KvSource, groups: int,
     m = _mass_struct(mass, mass_in, decay, int(mass_rows), b, h, n_max)
     lib = _lib.load()
     rows_max = max(0, min(int(rows_max), t))
-    need = lib.pqhsa_prompt_attend_workspace_bytes(t, b, h, groups, n_max, rows_max, dtype_code(kv.dtype), int(lse is not None))
+    need = lib.pqhsa_prompt_attend_workspace_bytes(t, b, h, groups, n_max, rows_max, dtype_code(kv.dtype), int(mass is not None))
     with _on_device(device):
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         rc = lib.pqhsa_prompt_attend_paged(q.data_ptr(), dtype_code(q.dtype), *_row_strides(q), out.data_ptr(),
