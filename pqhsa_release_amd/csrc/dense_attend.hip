@@ -291,12 +291,12 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_attend_kernel(DenseArg
 }
 
 // ---- join of the split partials: one workgroup per row -------------------------------------
-// Eight groups of 32 lanes (four dims a lane) take every eighth split, eight of them at a time with all
-// loads in flight at once: few rows join, so the time is one or two round trips to memory.  Each group
-// keeps a running maximum and sum; the groups meet in LDS.
-template <int DT>
+// Eight groups of 32 lanes (four dims a lane) take every eighth split, `kBatch` of them at a time with all
+// loads in flight at once: the time is one or two round trips to memory.  Each group keeps a running
+// maximum and sum; the groups meet in LDS.
+template <int DT, int kBatch>
 __global__ __launch_bounds__(256) void dense_join_kernel(JoinArgs a) {
-    constexpr int kGroups = 8, kBatch = 8;
+    constexpr int kGroups = 8;
     __shared__ float red[kGroups][kD];
     __shared__ float2 red_ml[kGroups];
     const int64_t r = blockIdx.x;
@@ -362,7 +362,9 @@ __global__ __launch_bounds__(256) void dense_join_kernel(JoinArgs a) {
 }
 
 int launch_join(const JoinArgs &a, int dtype, int64_t rows, hipStream_t stream) {
-    PQHSA_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL(dense_join_kernel<DT>, dim3((unsigned)rows), dim3(256), 0, stream, a));
+    PQHSA_DISPATCH_DTYPE(dtype,
+                         if (a.splits <= 16) hipLaunchKernelGGL((dense_join_kernel<DT, 2>), dim3((unsigned)rows), dim3(256), 0, stream, a);
+                         else hipLaunchKernelGGL((dense_join_kernel<DT, 8>), dim3((unsigned)rows), dim3(256), 0, stream, a));
     return check_launch("dense_join");
 }
 

@@ -107,6 +107,10 @@ __device__ inline uint32_t finite_part(uint32_t w) {
     }
 }
 
+__device__ inline uint64_t uniform(uint64_t x) {         // the same in every lane
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32)) << 32;
+}
+
 // 16 bytes per lane from memory into LDS at the wave-uniform byte address `lds` plus 16 * lane, without
 // passing through registers.  The compiler does not see the access: whoever reads the LDS waits with
 // direct_loads_done() and a barrier first.  (M0, which holds the LDS address, has no other use here.)
@@ -145,7 +149,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     int32_t *kdoc = phys + kSlots * 64;                                            // [slots][64] documents
     uint64_t *valid = reinterpret_cast<uint64_t *>(kdoc + kSlots * 64);            // [slots] rows that exist
     int32_t *tiles = reinterpret_cast<int32_t *>(valid + kSlots);                  // [slots] tile of the walk (documents)
-    int32_t *poison = tiles + kSlots;                                              // [2]: an infinity or NaN was set aside
+    int32_t *poison = tiles + kSlots;                                              // [2]: a sum is not finite; values were set aside
     uint32_t *wanted = reinterpret_cast<uint32_t *>(poison + 4);                   // [mask_words] tiles to walk
     uint32_t *pure = wanted + a.mask_words;                                        // [mask_words] tiles of the rows' one document
     const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char *)lds;
@@ -201,40 +205,55 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     const int t_begin = min(split * per, count), t_end = min(t_begin + per, count);
     auto key_tile = [&](int t) { return (t < walk_a ? t : walk_b + t - walk_a) * KT; };
 
+    // query rows as the second operand: lane (n, kg) holds row n
+    u32x4 qf[kSlices];
+    {
+        const char *p = a.q + ((rows.first + token) * a.q_row + (int64_t)(h * a.G + g) * a.q_head) * a.kv.esize;
+#pragma unroll
+        for (int u = 0; u < kSlices; ++u) qf[u] = *reinterpret_cast<const u32x4 *>(p + (u * 2 + kg) * 16);
+    }
+
     if (docs && t_begin < t_end) {
         // a bit per tile of the walk: some key lies in the rows' documents; every key is of their one document
-        int d_lo = 0x7fffffff, d_hi = -0x7fffffff - 1;
-        for (int p = max(wg_lo, 0) + lane; p <= wg_hi; p += 64) { d_lo = min(d_lo, docs[p]); d_hi = max(d_hi, docs[p]); }
-#pragma unroll
-        for (int x = 32; x > 0; x >>= 1) { d_lo = min(d_lo, __shfl_xor(d_lo, x, kWave)); d_hi = max(d_hi, __shfl_xor(d_hi, x, kWave)); }
-        constexpr int kPer = 64 / KT;                    // tiles a wave looks at per load
+        constexpr int kTokens = kPromptRows / 64, kPer = 64 / KT, kBatch = 8 / kPer;   // (8 tiles a wave and turn)
         constexpr uint64_t kAll = KT == 64 ? ~0ull : 0xffffffffull;
-        for (int w = wave; w * 32 < t_end - t_begin; w += WAVES) {
-            uint32_t some = 0, whole = 0;
+        int d_lo = 0x7fffffff, d_hi = -0x7fffffff - 1, own[kTokens];
+#pragma unroll
+        for (int i = 0; i < kTokens; ++i) own[i] = docs[max(min(wg_lo + i * 64 + lane, wg_hi), 0)];
 #pragma unroll 1
-            for (int x0 = 0; x0 < 32; x0 += 16) {
-                int d[16 / kPer];
-                bool in[16 / kPer];
+        for (int w = wave; w * 8 < t_end - t_begin; w += WAVES) {
+            int d[kBatch];
+            bool in[kBatch];
 #pragma unroll
-                for (int x = 0; x < 16 / kPer; ++x) {
-                    const int t = t_begin + w * 32 + x0 + x * kPer + lane / KT;
-                    const int j = key_tile(t) + lane % KT;
-                    in[x] = t < t_end && j < len;
-                    d[x] = in[x] ? docs[j] : 0;
-                }
+            for (int x = 0; x < kBatch; ++x) {
+                const int t = t_begin + w * 8 + x * kPer + lane / KT;
+                const int j = key_tile(t) + lane % KT;
+                in[x] = t < t_end && j < len;
+                d[x] = docs[in[x] ? j : 0];
+            }
+            if (w == wave) {
 #pragma unroll
-                for (int x = 0; x < 16 / kPer; ++x) {
-                    const uint64_t hit = __ballot(in[x] && d[x] >= d_lo && d[x] <= d_hi);
-                    const uint64_t same = __ballot(in[x] && d[x] == d_lo && d_lo == d_hi);
+                for (int i = 0; i < kTokens; ++i) { d_lo = min(d_lo, own[i]); d_hi = max(d_hi, own[i]); }
+                constexpr uint32_t kSign = 0x80000000u;    // (the order of the bits is then that of the numbers)
+                d_hi = (int)(wave_max_u32((uint32_t)d_hi ^ kSign) ^ kSign);
+                d_lo = (int)(~wave_max_u32(~((uint32_t)d_lo ^ kSign)) ^ kSign);
+            }
+            uint32_t some = 0, whole = 0;
 #pragma unroll
-                    for (int y = 0; y < kPer; ++y) {
-                        const int bit = x0 + x * kPer + y;
-                        if ((hit >> (y * 32)) & kAll) some |= 1u << bit;
-                        if (((same >> (y * 32)) & kAll) == kAll) whole |= 1u << bit;
-                    }
+            for (int x = 0; x < kBatch; ++x) {
+                const uint64_t hit = __ballot(in[x] && d[x] >= d_lo && d[x] <= d_hi);
+                const uint64_t same = __ballot(in[x] && d[x] == d_lo && d_lo == d_hi);
+#pragma unroll
+                for (int y = 0; y < kPer; ++y) {
+                    if ((hit >> (y * 32)) & kAll) some |= 1u << (x * kPer + y);
+                    if (((same >> (y * 32)) & kAll) == kAll) whole |= 1u << (x * kPer + y);
                 }
             }
-            if (lane == 0) { wanted[w] = some; pure[w] = whole; }
+            // (bits behind the last tile, in this byte's word or not written at all, are never looked at)
+            if (lane == 0) {
+                reinterpret_cast<uint8_t *>(wanted)[w] = (uint8_t)some;
+                reinterpret_cast<uint8_t *>(pure)[w] = (uint8_t)whole;
+            }
         }
         __syncthreads();
     }
@@ -270,16 +289,6 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
         return one_doc && (t < w.pre || (t >= w.from && t < w.to));
     };
 
-    // query rows as the second operand: lane (n, kg) holds row n
-    u32x4 qf[kSlices];
-    {
-        const char *p = a.q + ((rows.first + token) * a.q_row + (int64_t)(h * a.G + g) * a.q_head) * a.kv.esize;
-#pragma unroll
-        for (int u = 0; u < kSlices; ++u) qf[u] = *reinterpret_cast<const u32x4 *>(p + (u * 2 + kg) * 16);
-        // waited for here: inside the loop the compiler's wait would also be one for the direct loads in flight
-#pragma unroll
-        for (int u = 0; u < kSlices; ++u) asm volatile("" : "+v"(qf[u]));
-    }
     const float slope2 = GENERAL && a.score.slopes ? a.score.slopes[h * a.G + g] * kLog2e : 0.0f;
     const int row_doc = docs && pos >= 0 ? docs[pos] : 0;
     const int row_prefix = pos >= 0 ? prefix_all : 0;
@@ -338,8 +347,9 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     };
     auto fetch_keys = [&](int x) { fetch(a.kv.k_base, x, (x & (kStages - 1)) * kTileBytes, false); };
     auto fetch_values = [&](int x) { fetch(a.kv.v_base, x, kVat + (x & (kStages - 1)) * kTileBytes, true); };
-    // A tile that some rows of the workgroup do not see whole: a weight of zero would not cancel an infinite
-    // or NaN value, so these are set aside (and come back at the end, for the rows that see them).
+    // A weight of zero does not cancel an infinite or NaN value.  The walk is made without a thought for that;
+    // where a sum then is not finite it is made again, with such values set aside in the tiles that some
+    // rows of the workgroup do not see whole (they come back at the end, for the rows that see them).
     auto set_aside = [&](char *vl) {
         bool bad = false;
 #pragma unroll
@@ -354,16 +364,12 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
                 bad = true;
             }
         }
-        if (bad) poison[0] = 1;
+        if (bad) poison[1] = 1;
         __syncthreads();
     };
 
-    float m = -INFINITY, l = 0.0f;
+    float m, l;
     f32x16 acc[4];                                       // dim 32 dt + 8 (r / 4) + 4 kg + r % 4 of row n in acc[dt][r]
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[dt][r] = 0.0f;
     // where GENERAL is false scores stay unscaled, the scale goes into the exponent
     const float unit = GENERAL ? 1.0f : a.score.scale2;
 
@@ -402,28 +408,30 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
                               - slope2 * (float)abs(pos - j);
                 }
         }
-        const uint64_t exist = valid[slot];
+        const uint64_t exist = uniform(valid[slot]);
         if (all_see(t, wave_whole) && exist == (KT == 64 ? ~0ull : 0xffffffffull)) return;
-        // (bitwise, not short-circuit: a branch per key costs more than the comparisons)
+        // the row's keys as bits: [row_from, pos] and [0, row_prefix), those of its document, those that exist
+        auto below = [&](int j) { const int x = min(max(j - k0, 0), 64); return x == 0 ? 0ull : ~0ull >> (64 - x); };
+        uint64_t see = ((below(pos + 1) & ~below(row_from)) | below(row_prefix)) & exist;
+        if (docs) {                                      // one turn per document in the tile, mostly one or two
+            const int kd = kdoc[slot * 64 + lane];
+            uint64_t left = exist, own = 0;
+            while (left) {
+                const int d = __builtin_amdgcn_readlane(kd, __ffsll((unsigned long long)left) - 1);
+                const uint64_t hit = __ballot(kd == d);
+                own = d == row_doc ? hit : own;
+                left &= ~hit;
+            }
+            see &= own;
+        }
 #pragma unroll
         for (int T = 0; T < kTT; ++T) {
-            const uint32_t ok = (uint32_t)(exist >> (32 * T)) >> (4 * kg);
-            uint32_t seen = 0;
+            const uint32_t seen = (uint32_t)(see >> (32 * T)) >> (4 * kg);
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                int4 kd = make_int4(0, 0, 0, 0);
-                if (docs) kd = *reinterpret_cast<const int4 *>(&kdoc[slot * 64 + T * 32 + 8 * r4 + 4 * kg]);
-                const int d[4] = {kd.x, kd.y, kd.z, kd.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = k0 + T * 32 + 8 * r4 + 4 * kg + e;
-                    const uint32_t see = ((j >= row_from) & (j <= pos)) | (j < row_prefix);
-                    seen |= (docs ? see & (d[e] == row_doc) : see) << (8 * r4 + e);
-                }
+            for (int r = 0; r < 16; ++r) {
+                const uint32_t keep = (uint32_t)((int32_t)(seen << (31 - (8 * (r / 4) + r % 4))) >> 31);   // all ones: seen
+                s[T][r] = __uint_as_float((__float_as_uint(s[T][r]) & keep) | (0xff800000u & ~keep));
             }
-            seen &= ok;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[T][r] = (seen >> (8 * (r / 4) + r % 4)) & 1 ? s[T][r] : -INFINITY;
         }
     };
     auto largest = [&](const f32x16 (&s)[kTT]) {
@@ -499,54 +507,76 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     // arrived by the end of iteration x + stages - 2.  Tile x's own slot is still being read (its documents),
     // so the first that may be looked up anew is the one of tile x - 1.
     constexpr int kInFlight = (kStages - 2) * 2 * kLoads;
-    if (tid == 0) poison[0] = 0;
-    int t = next(t_begin), reach = t;
-    f32x16 s[kTT];
-    if (t < t_end) {
-        for (int x = 0; x < wave; ++x) reach = next(reach + 1);
-        if (wave < kSlots - 1) look_up(wave, reach);     // (as many waves as slots; the last slot is iteration 0's)
-        direct_loads_done<0>();
-        if (wave < kSlots - 1) resolve(wave, reach);
-        __syncthreads();
-        if (docs && wave == 0) reach = tile_at(kSlots - 2);
-        fetch_keys(0);
-        fetch_values(0);
-#pragma unroll
-        for (int x = 1; x < kStages - 1; ++x) { fetch_keys(x); fetch_values(x); }
-        direct_loads_done<kInFlight>();
-        __syncthreads();
-        if (!all_see(t, wg_whole)) set_aside(lds + kVat);
-    }
+    if (tid < 2) poison[tid] = 0;
+    const int t_first = next(t_begin);
 #pragma unroll 1
-    for (int x = 0; t < t_end; ++x) {
-        const int t1 = tile_at(x + 1);
-        const char *kl = lds + (x & (kStages - 1)) * kTileBytes;
-        char *vl = lds + kVat + (x & (kStages - 1)) * kTileBytes;
-        uint4 pw[kSteps];
-        fetch_keys(x + kStages - 1);
-        fetch_values(x + kStages - 1);
-        score_product(kl, s);
-        finish_scores(s, t, x & (kSlots - 1));
-        raise_maximum(largest(s));
-        weigh(s, pw);
-        value_product(lds0 + (uint32_t)(vl - lds), pw);
-        if (wave == 0) {
-            if (x + kStages >= kSlots - 1) resolve(x + kStages, tile_at(x + kStages));
-            if (docs) reach = next(reach + 1);
-            look_up(x + kSlots - 1, docs ? reach : min(t_begin + x + kSlots - 1, t_end));
-        }
-        if (t1 < t_end) {
+    for (bool careful = false;; careful = true) {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[dt][r] = 0.0f;
+        int t = t_first, reach = t;
+        f32x16 s[kTT];
+        if (t < t_end) {
+            for (int x = 0; x < wave; ++x) reach = next(reach + 1);
+            if (wave < kSlots - 1) look_up(wave, reach);     // (as many waves as slots; the last slot is iteration 0's)
+            // the query rows with them: inside the loop the compiler's wait would also be one for the direct loads
+#pragma unroll
+            for (int u = 0; u < kSlices; ++u) asm volatile("" : "+v"(qf[u]));
+            direct_loads_done<0>();
+            if (wave < kSlots - 1) resolve(wave, reach);
+            __syncthreads();
+            if (docs && wave == 0) reach = tile_at(kSlots - 2);
+            fetch_keys(0);
+            fetch_values(0);
+#pragma unroll
+            for (int x = 1; x < kStages - 1; ++x) { fetch_keys(x); fetch_values(x); }
             direct_loads_done<kInFlight>();
             __syncthreads();
-            if (!all_see(t1, wg_whole)) set_aside(lds + kVat + ((x + 1) & (kStages - 1)) * kTileBytes);
+            if (careful && !all_see(t, wg_whole)) set_aside(lds + kVat);
         }
-        t = t1;
-    }
-    direct_loads_done<0>();                              // (no load may reach the LDS after the workgroup has left it)
-    l += __shfl_xor(l, 32, kWave);
-    if (t_begin < t_end && poison[0]) {                  // the infinities and NaN that were set aside
 #pragma unroll 1
-        for (t = next(t_begin); t < t_end; t = next(t + 1)) {
+        for (int x = 0; t < t_end; ++x) {
+            const int t1 = tile_at(x + 1);
+            const char *kl = lds + (x & (kStages - 1)) * kTileBytes;
+            char *vl = lds + kVat + (x & (kStages - 1)) * kTileBytes;
+            uint4 pw[kSteps];
+            fetch_keys(x + kStages - 1);
+            fetch_values(x + kStages - 1);
+            score_product(kl, s);
+            finish_scores(s, t, x & (kSlots - 1));
+            raise_maximum(largest(s));
+            weigh(s, pw);
+            value_product(lds0 + (uint32_t)(vl - lds), pw);
+            if (wave == 0) {
+                if (x + kStages >= kSlots - 1) resolve(x + kStages, tile_at(x + kStages));
+                if (docs) reach = next(reach + 1);
+                look_up(x + kSlots - 1, docs ? reach : min(t_begin + x + kSlots - 1, t_end));
+            }
+            if (t1 < t_end) {
+                direct_loads_done<kInFlight>();
+                __syncthreads();
+                if (careful && !all_see(t1, wg_whole)) set_aside(lds + kVat + ((x + 1) & (kStages - 1)) * kTileBytes);
+            }
+            t = t1;
+        }
+        direct_loads_done<0>();                              // (no load may reach the LDS after the workgroup has left it)
+        if (careful || t_first >= t_end) break;
+        bool finite = true;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) finite = finite & (fabsf(acc[dt][r]) < INFINITY);
+        if (!finite) poison[0] = 1;
+        __syncthreads();                                 // (the ring is no longer read, either)
+        if (!poison[0]) break;
+    }
+    l += __shfl_xor(l, 32, kWave);
+    if (t_first < t_end && poison[1]) {                  // the infinities and NaN that were set aside
+#pragma unroll 1
+        for (int t = t_first; t < t_end; t = next(t + 1)) {
             const int k0 = key_tile(t);
             if (all_see(t, wg_whole)) continue;
 #pragma unroll 1
@@ -607,12 +637,17 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
 constexpr int kMassWaves = 4;
 
 template <int DT>
-__global__ __launch_bounds__(kMassWaves * kWave, 2) void prompt_mass_kernel(PromptArgs a) {
+__global__ __launch_bounds__(kMassWaves * kWave, DT == PQHSA_F32 ? 2 : 3) void prompt_mass_kernel(PromptArgs a) {
     constexpr bool kF32 = DT == PQHSA_F32;
     constexpr int kRowBytes = kD * (kF32 ? 4 : 2), kSlices = kRowBytes / 32, kRowLanes = kRowBytes / 16, kPass = 64 / kRowLanes;
     constexpr int kTile = 32 * kRowBytes, kLoads = kTile / 1024 / kMassWaves;
-    __shared__ __align__(16) char tiles[2 * kTile];
+    // A ring of four tiles, each with the (m, l) of its rows: three are on their way while one is computed (with
+    // one on its way every tile took the whole round trip to the L2).
+    constexpr int kRing = 4;
+    __shared__ __align__(16) char tiles[kRing * kTile];
+    __shared__ float2 sums[kRing][32];
     const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char *)tiles;
+    const uint32_t sums0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char *)reinterpret_cast<char *>(&sums[0][0]);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n = lane & 31, kg = lane >> 5;
     const int b = blockIdx.y / a.H, h = blockIdx.y - b * a.H;
@@ -647,8 +682,16 @@ __global__ __launch_bounds__(kMassWaves * kWave, 2) void prompt_mass_kernel(Prom
             const char *p = a.q + ((rows.first + token) * a.q_row + (int64_t)(h * a.G + pr - token * a.G) * a.q_head) * a.kv.esize;
             load_direct(lds0 + buf * kTile + (wave * kLoads + i) * 1024, p + ((lane % kRowLanes) ^ (r & 15)) * 16);
         }
+        if (wave == 0) {
+            const int pr = min(at + lane / 2, packed - 1), token = token_of(pr);
+            const float2 *p = a.row_ml + (rows.first + token) * (int64_t)(a.H * a.G) + h * a.G + pr - token * a.G;
+            load_direct4(sums0 + buf * 256, reinterpret_cast<const float *>(p) + (lane & 1));
+        }
     };
-    if (at < packed) fetch(at, 0);
+    if (at < packed) {
+#pragma unroll
+        for (int i = 0; i < kRing - 1; ++i) fetch(at + i * 32, i);
+    }
 
     uint4 kf[kSlices];
     const int64_t off = k0 + n < len ? checked_row_bytes(a.kv, a.blocks, b, h, k0 + n) : -1;
@@ -663,14 +706,15 @@ __global__ __launch_bounds__(kMassWaves * kWave, 2) void prompt_mass_kernel(Prom
     direct_loads_done<0>();
     __syncthreads();
 
-    for (int buf = 0; at < packed; at += 32, buf ^= 1) {
+    for (int buf = 0; at < packed; at += 32, buf = (buf + 1) % kRing) {
         // past the window of all the workgroup's keys, and these are not in the prefix: no later row sees them
         const int first_row = first_pos + token_of(at);
         if (wg_k0 >= prefix && first_row - wg_last >= window) break;
-        if (at + 32 < packed) fetch(at + 32, buf ^ 1);
-        const bool mine = at + n < packed;
+        fetch(at + (kRing - 1) * 32, (buf + kRing - 1) % kRing);      // (behind the last row: the last row again)
+        const float2 ml = sums[buf][n];
+        const bool gives = at + n < packed && ml.y != 0.0f;            // m = +inf: the row gives no weight
+        const float m = gives ? ml.x : INFINITY, inv = gives ? 1.0f / ml.y : 0.0f;
         const int pr = min(at + n, packed - 1), token = token_of(pr), g = pr - token * a.G, pos = first_pos + token;
-        const float2 ml = a.row_ml[(rows.first + token) * (int64_t)(a.H * a.G) + h * a.G + g];
         f32x16 s;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.0f;
@@ -685,8 +729,6 @@ __global__ __launch_bounds__(kMassWaves * kWave, 2) void prompt_mass_kernel(Prom
                 s = Half16<DT>::mfma32(kf[u], x, s);
             }
         }
-        const bool gives = mine && ml.y != 0.0f;
-        const float m = gives ? ml.x : INFINITY, inv = gives ? 1.0f / ml.y : 0.0f;
         const int last_row = first_pos + token_of(min(at + 31, packed - 1));
         if (!general && ok == ~0u && first_row >= k0 + 31 && last_row - k0 < window) {   // every row sees every key
 #pragma unroll
@@ -705,7 +747,7 @@ __global__ __launch_bounds__(kMassWaves * kWave, 2) void prompt_mass_kernel(Prom
                 sum[r] = __builtin_fmaf(see & 1 ? exp2_fast(z - m) : 0.0f, inv, sum[r]);
             }
         }
-        direct_loads_done<0>();
+        direct_loads_done<(kRing - 2) * kLoads>();
         __syncthreads();
     }
     direct_loads_done<0>();
@@ -738,7 +780,7 @@ PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint,
     PromptPlan p = {};
     // Eight waves (256 rows, four stages, one workgroup per compute unit) halve the K/V traffic of four (128
     // rows, two stages, two workgroups), which overlap each other's starts and ends.
-    p.waves = T * G / 256 * H >= 512 ? 8 : 4;
+    p.waves = T * G / 256 * H >= (getenv("PQ_W") ? atoi(getenv("PQ_W")) : 512) ? 8 : 4;
     const int tile_rows = p.waves * 32;
     p.tiles = (T * G + tile_rows - 1) / tile_rows + B;              // every sequence may end inside a tile
     int64_t busy = p.tiles - B;
@@ -750,7 +792,7 @@ PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint,
     // fill the chip with keys enough a workgroup to be worth the join (a launch and the partial sums' way
     // through memory, 8 us: eight tiles of the 2-byte types, two of fp32 take that long)
     const int64_t want = ((p.waves == 8 ? 256 : 512) + busy * H - 1) / (busy * H);
-    const int64_t least = key_tile == 32 ? 64 : 512;
+    const int64_t least = key_tile == 32 ? (getenv("PQ_L") ? atoi(getenv("PQ_L")) : 64) : (getenv("PQ_M") ? atoi(getenv("PQ_M")) : 512);
     const int64_t most = ((int64_t)n_max + least - 1) / least;
     p.splits = (int)(want < most ? want : most);
     if (p.splits < 1) p.splits = 1;
@@ -819,7 +861,7 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
     if (kv->paged)
         PQHSA_REQUIRE(blocks > 0 && (int64_t)kv->max_blocks * kv->block_size >= n_max,
                       "%s: %d blocks, and a table of %d x %d tokens for n_max %d", what, blocks, kv->max_blocks, kv->block_size, n_max);
-    PQHSA_REQUIRE(T * G < 0x7fffffff && T * H * G < 0x7fffffff, "%s: %lld rows of %d x %d heads are too many", what, (long long)T, H, G);
+    PQHSA_REQUIRE(T * G < 0x7fffffff - 65536 && T * H * G < 0x7fffffff, "%s: %lld rows of %d x %d heads are too many", what, (long long)T, H, G);
     PQHSA_REQUIRE((int64_t)B * H <= 65535, "%s: too many sequences and heads", what);
     const int key_tile = kv->dtype == PQHSA_F32 ? 32 : 64;
     const PromptPlan p = plan_prompt(T, B, H, G, n_max, rows_hint, key_tile, mass != nullptr);
