@@ -416,7 +416,10 @@ __global__ __launch_bounds__(256) void dense_mass_kernel(MassArgs a) {
         float w = a.in ? a.decay * a.in[(int64_t)bh * a.stride + j] : 0.0f;
         const int v = j < range.first ? j : j - range.gap;
         if (j < range.first || v >= range.first)
-            for (int g = 0; g < a.G; ++g) w = __builtin_fmaf(exp2_fast(scores[g * a.score_stride + v] - row[g].x), row[g].y, w);
+            for (int g = 0; g < a.G; ++g) {
+                const float z = scores[g * a.score_stride + v];
+                w += z == -INFINITY ? 0.0f : exp2_fast(z - row[g].x) * row[g].y;   // (-inf: masked, also from a row of NaN)
+            }
         a.out[(int64_t)bh * a.stride + j] = w;
     }
 }

@@ -22,6 +22,7 @@ constexpr int kEvictLoads = 16;                          // keys per thread, all
 constexpr int kEvictChunk = kEvictThreads * kEvictLoads;
 constexpr int kEvictCopies = 8;                          // histogram copies, by lane: a wave's equal digits rarely meet
 constexpr int kEvictBins = 2048;
+constexpr int kEvictStride = kEvictBins + 8;             // words of a copy: the copies of a bin lie in different banks
 constexpr int kMoveThreads = 256;
 constexpr int kMoveRows = 64;                            // kept keys per workgroup of the move
 
@@ -58,7 +59,7 @@ __device__ inline EvictStream evict_stream(const EvictArgs &a, int b) {
 }
 
 struct EvictLds {
-    uint4 copies[kEvictBins * kEvictCopies / 4];
+    uint2 copies[kEvictCopies][kEvictStride / 2];
     uint32_t found[2];
     uint32_t wave_sums[kEvictThreads / kWave];
 };
@@ -77,30 +78,35 @@ __device__ inline void load_chunk(const float *mass, int j0, int len, float (&w)
 }
 
 __device__ inline void clear_copies(EvictLds &l) {
-    for (int x = threadIdx.x; x < kEvictBins * kEvictCopies / 4; x += kEvictThreads) l.copies[x] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int c = 0; c < kEvictCopies; ++c) l.copies[c][threadIdx.x] = make_uint2(0u, 0u);
 }
 
 // adds the digits of the chunk's candidates, those that share `prefix` above the digit (copies cleared, barriers outside)
 __device__ inline void count_digits(EvictLds &l, const float (&w)[kEvictLoads], int j0, const EvictStream &s, int pass, uint32_t prefix) {
-    uint32_t *copies = reinterpret_cast<uint32_t *>(l.copies) + (threadIdx.x & (kEvictCopies - 1));
+    uint32_t *copy = reinterpret_cast<uint32_t *>(l.copies[threadIdx.x & (kEvictCopies - 1)]);
     const int shift = digit_shift(pass), above = shift + digit_bits(pass);
 #pragma unroll
     for (int e = 0; e < kEvictLoads; ++e) {
         const int j = chunk_key(j0, e);
         const uint32_t k = order_key(w[e]);
         if (j >= s.low && j < s.high && (pass == 0 || (k >> above) == prefix))
-            atomicAdd(&copies[((k >> shift) & ((1u << digit_bits(pass)) - 1u)) * kEvictCopies], 1u);
+            atomicAdd(&copy[(k >> shift) & ((1u << digit_bits(pass)) - 1u)], 1u);
     }
 }
 
-// A thread owns two neighbouring bins, thread 0 the highest two: (higher, lower).
+// A thread owns two neighbouring bins, thread 0 the highest two: (higher, lower).  Read, they are cleared for the
+// next digit.
 __device__ inline int high_bin() { return kEvictBins - 1 - 2 * (int)threadIdx.x; }
-__device__ inline uint2 fold_copies(const EvictLds &l) {
-    uint2 r;
-    const int hi = high_bin();
-    const uint4 a = l.copies[2 * hi], b = l.copies[2 * hi + 1], c = l.copies[2 * hi - 2], d = l.copies[2 * hi - 1];
-    r.x = a.x + a.y + a.z + a.w + b.x + b.y + b.z + b.w;
-    r.y = c.x + c.y + c.z + c.w + d.x + d.y + d.z + d.w;
+__device__ inline uint2 fold_copies(EvictLds &l) {
+    uint2 r = make_uint2(0u, 0u);
+#pragma unroll
+    for (int c = 0; c < kEvictCopies; ++c) {
+        uint2 &x = l.copies[c][high_bin() / 2];
+        r.x += x.y;
+        r.y += x.x;
+        x = make_uint2(0u, 0u);
+    }
     return r;
 }
 
@@ -193,10 +199,10 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a
     write_rest(a, bh, b, s.len);
     uint32_t prefix = 0, want = s.want;
     if (want > 0) {
+        clear_copies(l);
+        __syncthreads();
 #pragma unroll
         for (int pass = 0; pass < 3; ++pass) {
-            clear_copies(l);
-            __syncthreads();
             count_digits(l, w, 0, s, pass, prefix);
             __syncthreads();
             find_cut(l, fold_copies(l), want);

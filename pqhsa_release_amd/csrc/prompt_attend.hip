@@ -16,6 +16,8 @@
 // Tiles no row of the workgroup sees are left out of the walk (causal order, window, prefix from the
 // positions; documents from a bit per tile); a tile every row sees skips all mask arithmetic.  Where the
 // launch would not fill the chip the key range is split over workgroups and joined by a second launch.
+#include <atomic>
+
 #include "dense_common.h"
 
 namespace pqhsa {
@@ -110,6 +112,27 @@ __device__ inline uint32_t finite_part(uint32_t w) {
 __device__ inline uint64_t uniform(uint64_t x) {         // the same in every lane
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32)) << 32;
 }
+
+// The keys k0 .. k0 + 63 that a lane's query row sees, as bits: [row_from, pos] and [0, row_prefix), of these
+// the ones that `exist` (the same in every lane) and, with documents, the ones of its own; kd is the
+// document of key k0 + lane.
+__device__ inline uint64_t seen_keys(int k0, uint64_t exist, int pos, int row_from, int row_prefix, bool docs, int kd, int row_doc) {
+    auto below = [&](int j) { const int x = min(max(j - k0, 0), 64); return x == 0 ? 0ull : ~0ull >> (64 - x); };
+    uint64_t see = ((below(pos + 1) & ~below(row_from)) | below(row_prefix)) & exist;
+    if (docs) {                                          // one turn per document among the keys, mostly one or two
+        uint64_t left = exist, own = 0;
+        while (left) {
+            const int d = __builtin_amdgcn_readlane(kd, __ffsll((unsigned long long)left) - 1);
+            const uint64_t hit = __ballot(kd == d);
+            own = d == row_doc ? hit : own;
+            left &= ~hit;
+        }
+        see &= own;
+    }
+    return see;
+}
+// all ones where a lane's key r of 16 (bit 8 (r / 4) + r % 4 of `seen`) is seen
+__device__ inline uint32_t seen_mask(uint32_t seen, int r) { return (uint32_t)((int32_t)(seen << (31 - (8 * (r / 4) + r % 4))) >> 31); }
 
 // 16 bytes per lane from memory into LDS at the wave-uniform byte address `lds` plus 16 * lane, without
 // passing through registers.  The compiler does not see the access: whoever reads the LDS waits with
@@ -410,27 +433,14 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
         }
         const uint64_t exist = uniform(valid[slot]);
         if (all_see(t, wave_whole) && exist == (KT == 64 ? ~0ull : 0xffffffffull)) return;
-        // the row's keys as bits: [row_from, pos] and [0, row_prefix), those of its document, those that exist
-        auto below = [&](int j) { const int x = min(max(j - k0, 0), 64); return x == 0 ? 0ull : ~0ull >> (64 - x); };
-        uint64_t see = ((below(pos + 1) & ~below(row_from)) | below(row_prefix)) & exist;
-        if (docs) {                                      // one turn per document in the tile, mostly one or two
-            const int kd = kdoc[slot * 64 + lane];
-            uint64_t left = exist, own = 0;
-            while (left) {
-                const int d = __builtin_amdgcn_readlane(kd, __ffsll((unsigned long long)left) - 1);
-                const uint64_t hit = __ballot(kd == d);
-                own = d == row_doc ? hit : own;
-                left &= ~hit;
-            }
-            see &= own;
-        }
+        const uint64_t see = seen_keys(k0, exist, pos, row_from, row_prefix, docs != nullptr, docs ? kdoc[slot * 64 + lane] : 0, row_doc);
 #pragma unroll
         for (int T = 0; T < kTT; ++T) {
             const uint32_t seen = (uint32_t)(see >> (32 * T)) >> (4 * kg);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const uint32_t keep = (uint32_t)((int32_t)(seen << (31 - (8 * (r / 4) + r % 4))) >> 31);   // all ones: seen
-                s[T][r] = __uint_as_float((__float_as_uint(s[T][r]) & keep) | (0xff800000u & ~keep));
+                const uint32_t keep = seen_mask(seen, r);
+                s[T][r] = __uint_as_float((__float_as_uint(s[T][r]) & keep) | (0xff800000u & ~keep));   // (-inf)
             }
         }
     };
@@ -629,20 +639,21 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
 
 // ---- weight of every key, summed over the last rows of the prompts -----------------------------
 // With every row's maximum m and sum l known the weights are one product K Q^T and an exp2 away (m and l
-// rather than the log-sum-exp: rounding that to fp32 would put 1e-6 of error on every weight).  A wave keeps 32
-// keys as the first operand in registers; the counted rows pass by in tiles of 32, which the four waves of
-// a workgroup share in LDS (a row's pieces lie 256 bytes apart for the lanes of an operand: read from
-// memory by every wave they took four times the requests).  Every lane sums its rows' weights of 16
-// keys, the lanes are summed at the end: no atomics, one owner per key.
+// rather than the log-sum-exp: rounding that to fp32 would put 1e-6 of error on every weight).  A wave keeps 64
+// keys (32 in fp32) as the first operand in registers; the counted rows pass by in tiles of 32, which the
+// four waves of a workgroup share in LDS (a row's pieces lie 256 bytes apart for the lanes of an operand:
+// read from memory by every wave they took four times the requests).  Every lane sums its rows' weights
+// of its keys, the lanes are summed at the end: no atomics, one owner per key.
 constexpr int kMassWaves = 4;
+constexpr int mass_keys(int dt) { return dt == PQHSA_F32 ? 32 : 64; }      // of a wave
 
 template <int DT>
-__global__ __launch_bounds__(kMassWaves * kWave, DT == PQHSA_F32 ? 2 : 3) void prompt_mass_kernel(PromptArgs a) {
+__global__ __launch_bounds__(kMassWaves * kWave, 2) void prompt_mass_kernel(PromptArgs a) {
     constexpr bool kF32 = DT == PQHSA_F32;
     constexpr int kRowBytes = kD * (kF32 ? 4 : 2), kSlices = kRowBytes / 32, kRowLanes = kRowBytes / 16, kPass = 64 / kRowLanes;
     constexpr int kTile = 32 * kRowBytes, kLoads = kTile / 1024 / kMassWaves;
-    // A ring of four tiles, each with the (m, l) of its rows: three are on their way while one is computed (with
-    // one on its way every tile took the whole round trip to the L2).
+    constexpr int kKeys = mass_keys(DT), kTT = kKeys / 32;
+    // A ring of four tiles, each with the (m, l) of its rows: three are on their way while one is computed.
     constexpr int kRing = 4;
     __shared__ __align__(16) char tiles[kRing * kTile];
     __shared__ float2 sums[kRing][32];
@@ -652,9 +663,9 @@ __global__ __launch_bounds__(kMassWaves * kWave, DT == PQHSA_F32 ? 2 : 3) void p
     const int n = lane & 31, kg = lane >> 5;
     const int b = blockIdx.y / a.H, h = blockIdx.y - b * a.H;
     const int len = __builtin_amdgcn_readfirstlane(sequence_length(a.seq_lens, b, a.n_max));
-    const int wg_k0 = blockIdx.x * kMassWaves * 32, k0 = wg_k0 + wave * 32;
+    const int wg_k0 = blockIdx.x * kMassWaves * kKeys, k0 = wg_k0 + wave * kKeys;
     if (wg_k0 >= len) return;
-    const int wg_last = min(wg_k0 + kMassWaves * 32, len) - 1;
+    const int wg_last = min(wg_k0 + kMassWaves * kKeys, len) - 1;
     PromptRows rows = sequence_rows(a.cu_rows, a.T, b);
     rows.first = __builtin_amdgcn_readfirstlane((int)rows.first);
     rows.rows = __builtin_amdgcn_readfirstlane(rows.rows);
@@ -673,97 +684,152 @@ __global__ __launch_bounds__(kMassWaves * kWave, DT == PQHSA_F32 ? 2 : 3) void p
         const int t = (int)__umulhi((uint32_t)pr, magic);
         return pr - t * a.G >= a.G ? t + 1 : t;
     };
-    // rows at .. at + 31 into LDS (pieces placed as the prompt kernel's K); rows past the end repeat the last
-    auto fetch = [&](int at, int buf) {
+    // A lane walks the rows it fetches 32 packed rows (step_tokens tokens and step_heads heads) at a time; behind
+    // the last row it fetches that one again, so that the number of loads in flight is always the same.
+    const int step_tokens = token_of(32), step_heads = 32 - step_tokens * a.G;
+    struct Walk { int pr, g; int64_t off; };             // packed row, its head in the group, where it lies
+    auto start = [&](int pr, int64_t row, int64_t head) {
+        const int token = token_of(pr), g = pr - token * a.G;
+        return Walk{pr, g, (rows.first + token) * row + (int64_t)(h * a.G + g) * head};
+    };
+    auto advance = [&](Walk &w, int64_t step, int64_t wrap) {
+        w.pr += 32;
+        w.g += step_heads;
+        w.off += step;
+        if (w.g >= a.G) { w.g -= a.G; w.off += wrap; }
+    };
+    const int64_t q_row = a.q_row * a.kv.esize, q_head = a.q_head * a.kv.esize;
+    const int64_t q_step = step_tokens * q_row + step_heads * q_head, q_wrap = q_row - a.G * q_head;
+    const int64_t ml_row = (int64_t)a.H * a.G, ml_step = step_tokens * ml_row + step_heads, ml_wrap = ml_row - a.G;
+    Walk walk[kLoads], ml_walk = {0, 0, 0};
+    int64_t q_last = 0, ml_last = 0;
+    auto fetch = [&](int buf) {                          // the next tile (pieces placed as the prompt kernel's K)
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int r = (wave * kLoads + i) * kPass + lane / kRowLanes;
-            const int pr = min(at + r, packed - 1), token = token_of(pr);
-            const char *p = a.q + ((rows.first + token) * a.q_row + (int64_t)(h * a.G + pr - token * a.G) * a.q_head) * a.kv.esize;
-            load_direct(lds0 + buf * kTile + (wave * kLoads + i) * 1024, p + ((lane % kRowLanes) ^ (r & 15)) * 16);
+            load_direct(lds0 + buf * kTile + (wave * kLoads + i) * 1024,
+                        a.q + (walk[i].pr < packed ? walk[i].off : q_last) + ((lane % kRowLanes) ^ (r & 15)) * 16);
+            advance(walk[i], q_step, q_wrap);
         }
         if (wave == 0) {
-            const int pr = min(at + lane / 2, packed - 1), token = token_of(pr);
-            const float2 *p = a.row_ml + (rows.first + token) * (int64_t)(a.H * a.G) + h * a.G + pr - token * a.G;
-            load_direct4(sums0 + buf * 256, reinterpret_cast<const float *>(p) + (lane & 1));
+            load_direct4(sums0 + buf * 256, reinterpret_cast<const float *>(a.row_ml + (ml_walk.pr < packed ? ml_walk.off : ml_last)) + (lane & 1));
+            advance(ml_walk, ml_step, ml_wrap);
         }
     };
     if (at < packed) {
+        q_last = start(packed - 1, q_row, q_head).off;
+        ml_last = start(packed - 1, ml_row, 1).off;
 #pragma unroll
-        for (int i = 0; i < kRing - 1; ++i) fetch(at + i * 32, i);
+        for (int i = 0; i < kLoads; ++i) walk[i] = start(at + (wave * kLoads + i) * kPass + lane / kRowLanes, q_row, q_head);
+        ml_walk = start(at + lane / 2, ml_row, 1);
+#pragma unroll
+        for (int i = 0; i < kRing - 1; ++i) fetch(i);
     }
 
-    uint4 kf[kSlices];
-    const int64_t off = k0 + n < len ? checked_row_bytes(a.kv, a.blocks, b, h, k0 + n) : -1;
+    const int key_doc = docs && lane < kKeys && k0 + lane < len ? docs[k0 + lane] : 0;
+    uint4 kf[kTT][kSlices];
+    uint64_t ok = 0;                                     // keys that exist, the same in every lane
 #pragma unroll
-    for (int u = 0; u < kSlices; ++u)
-        kf[u] = *reinterpret_cast<const uint4 *>(a.kv.k_base + (off < 0 ? 0 : off) + (u * 2 + kg) * 16);
-    const uint32_t ok = (uint32_t)__ballot(off >= 0);    // (both halves of the wave hold the same 32 keys)
+    for (int T = 0; T < kTT; ++T) {
+        const int64_t off = k0 + T * 32 + n < len ? checked_row_bytes(a.kv, a.blocks, b, h, k0 + T * 32 + n) : -1;
+#pragma unroll
+        for (int u = 0; u < kSlices; ++u)
+            kf[T][u] = *reinterpret_cast<const uint4 *>(a.kv.k_base + (off < 0 ? 0 : off) + (u * 2 + kg) * 16);
+        ok |= (uint64_t)(uint32_t)__ballot(off >= 0) << (32 * T);   // (both halves of the wave hold the same 32 keys)
+    }
     const bool general = a.score.capped || a.score.slopes || docs;
-    float sum[16];
+    float sum[kTT][16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sum[r] = 0.0f;
+    for (int T = 0; T < kTT; ++T)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[T][r] = 0.0f;
     direct_loads_done<0>();
     __syncthreads();
 
+#pragma unroll 1
     for (int buf = 0; at < packed; at += 32, buf = (buf + 1) % kRing) {
         // past the window of all the workgroup's keys, and these are not in the prefix: no later row sees them
         const int first_row = first_pos + token_of(at);
         if (wg_k0 >= prefix && first_row - wg_last >= window) break;
-        fetch(at + (kRing - 1) * 32, (buf + kRing - 1) % kRing);      // (behind the last row: the last row again)
+        fetch((buf + kRing - 1) % kRing);
         const float2 ml = sums[buf][n];
         const bool gives = at + n < packed && ml.y != 0.0f;            // m = +inf: the row gives no weight
         const float m = gives ? ml.x : INFINITY, inv = gives ? 1.0f / ml.y : 0.0f;
-        const int pr = min(at + n, packed - 1), token = token_of(pr), g = pr - token * a.G, pos = first_pos + token;
-        f32x16 s;
+        f32x16 s[kTT];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+        for (int T = 0; T < kTT; ++T)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[T][r] = 0.0f;
 #pragma unroll
         for (int u = 0; u < kSlices; ++u) {
             const uint4 x = *reinterpret_cast<const uint4 *>(tiles + buf * kTile + n * kRowBytes + (((u * 2 + kg) ^ (n & 15)) * 16));
-            if constexpr (kF32) {
-                const f32x4 y = __builtin_bit_cast(f32x4, kf[u]), z = __builtin_bit_cast(f32x4, x);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s = __builtin_amdgcn_mfma_f32_32x32x2f32(y[c], z[c], s, 0, 0, 0);
-            } else {
-                s = Half16<DT>::mfma32(kf[u], x, s);
+            for (int T = 0; T < kTT; ++T) {
+                if constexpr (kF32) {
+                    const f32x4 y = __builtin_bit_cast(f32x4, kf[T][u]), z = __builtin_bit_cast(f32x4, x);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) s[T] = __builtin_amdgcn_mfma_f32_32x32x2f32(y[c], z[c], s[T], 0, 0, 0);
+                } else {
+                    s[T] = Half16<DT>::mfma32(kf[T][u], x, s[T]);
+                }
             }
         }
         const int last_row = first_pos + token_of(min(at + 31, packed - 1));
-        if (!general && ok == ~0u && first_row >= k0 + 31 && last_row - k0 < window) {   // every row sees every key
+        if (!general && ok == (kTT == 2 ? ~0ull : 0xffffffffull) && first_row >= k0 + kKeys - 1 && last_row - k0 < window) {   // every row sees every key
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum[r] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[r], a.score.scale2, -m)), inv, sum[r]);
+            for (int T = 0; T < kTT; ++T)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    sum[T][r] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[T][r], a.score.scale2, -m)), inv, sum[T][r]);
         } else {
-            const float slope2 = a.score.slopes ? a.score.slopes[h * a.G + g] * kLog2e : 0.0f;
-            const int row_doc = docs && pos >= 0 ? docs[pos] : 0;
-            const int row_prefix = pos >= 0 ? prefix : 0, row_from = pos >= 0 ? max(pos - window + 1, 0) : 0x7fffffff;
+            const int pr = min(at + n, packed - 1), token = token_of(pr), g = pr - token * a.G, pos = first_pos + token;
+            const uint64_t see = seen_keys(k0, ok, pos, pos >= 0 ? max(pos - window + 1, 0) : 0x7fffffff, pos >= 0 ? prefix : 0,
+                                           docs != nullptr, key_doc, docs && pos >= 0 ? docs[pos] : 0);
+            // (one branch a rule, not one a key: few workgroups come here, but the others are done long before them)
+            float unit = a.score.scale2;
+            if (a.score.capped) {
+                unit = a.score.cap2;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int jj = 8 * (r / 4) + 4 * kg + r % 4, j = k0 + jj;
-                float z = a.score.capped ? a.score.cap2 * tanh_score(s[r] * a.score.in_cap) : s[r] * a.score.scale2;
-                z -= slope2 * (float)abs(pos - j);
-                uint32_t see = (((j >= row_from) & (j <= pos)) | (j < row_prefix)) & (ok >> jj);
-                if (docs) see &= j < len && docs[j] == row_doc;
-                sum[r] = __builtin_fmaf(see & 1 ? exp2_fast(z - m) : 0.0f, inv, sum[r]);
+                for (int T = 0; T < kTT; ++T)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[T][r] = tanh_score(s[T][r] * a.score.in_cap);
+            }
+            const float slope2 = a.score.slopes ? a.score.slopes[h * a.G + g] * kLog2e : 0.0f;
+#pragma unroll
+            for (int T = 0; T < kTT; ++T) {
+                const uint32_t seen = (uint32_t)(see >> (32 * T)) >> (4 * kg);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = k0 + T * 32 + 8 * (r / 4) + 4 * kg + r % 4;
+                    const float bias = __builtin_fmaf(slope2, (float)abs(pos - j), m);
+                    sum[T][r] += __uint_as_float(__float_as_uint(exp2_fast(__builtin_fmaf(s[T][r], unit, -bias)) * inv) & seen_mask(seen, r));
+                }
             }
         }
         direct_loads_done<(kRing - 2) * kLoads>();
         __syncthreads();
     }
     direct_loads_done<0>();
+    // Sums over the 32 lanes of each half, of 32 (16) keys at once: in every step a lane hands over the half of
+    // its keys that its partner keeps, so lane n ends up with key n (n % 16) of the half.
+    float x[kTT * 16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        float x = sum[r];
-        x += __shfl_xor(x, 1, kWave);
-        x += __shfl_xor(x, 2, kWave);
-        x += __shfl_xor(x, 4, kWave);
-        x += __shfl_xor(x, 8, kWave);
-        x += __shfl_xor(x, 16, kWave);
-        const int j = k0 + 8 * (r / 4) + 4 * kg + r % 4;
-        if (n == r && j < len) {                         // one lane of each half writes key r's sum
-            const int64_t o = (int64_t)blockIdx.y * a.mass_stride + j;
-            a.mass_out[o] = (a.mass_in ? a.decay * a.mass_in[o] : 0.0f) + x;
+    for (int i = 0; i < kTT * 16; ++i) x[i] = sum[i / 16][i % 16];
+    if constexpr (kTT == 1) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] += __shfl_xor(x[i], 16, kWave);
+    }
+#pragma unroll
+    for (int half = kTT * 8; half > 0; half /= 2)
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+            const float keep = n & half ? x[i + half] : x[i], give = n & half ? x[i] : x[i + half];
+            x[i] = keep + __shfl_xor(give, half, kWave);
         }
+    const int T = n / 16 % kTT, r = n % 16, j = k0 + T * 32 + 8 * (r / 4) + 4 * kg + r % 4;
+    if (n < kTT * 16 && j < len) {
+        const int64_t o = (int64_t)blockIdx.y * a.mass_stride + j;
+        a.mass_out[o] = (a.mass_in ? a.decay * a.mass_in[o] : 0.0f) + x[0];
     }
 }
 
@@ -778,9 +844,10 @@ struct PromptPlan {
 
 PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint, int key_tile, bool mass) {
     PromptPlan p = {};
+    p.splits = 1;
     // Eight waves (256 rows, four stages, one workgroup per compute unit) halve the K/V traffic of four (128
     // rows, two stages, two workgroups), which overlap each other's starts and ends.
-    p.waves = T * G / 256 * H >= (getenv("PQ_W") ? atoi(getenv("PQ_W")) : 512) ? 8 : 4;
+    p.waves = T * G / 256 * H >= 512 ? 8 : 4;
     const int tile_rows = p.waves * 32;
     p.tiles = (T * G + tile_rows - 1) / tile_rows + B;              // every sequence may end inside a tile
     int64_t busy = p.tiles - B;
@@ -789,13 +856,20 @@ PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint,
         if (each * B > busy) busy = each * B;
     }
     if (busy < 1) busy = 1;
-    // fill the chip with keys enough a workgroup to be worth the join (a launch and the partial sums' way
-    // through memory, 8 us: eight tiles of the 2-byte types, two of fp32 take that long)
-    const int64_t want = ((p.waves == 8 ? 256 : 512) + busy * H - 1) / (busy * H);
-    const int64_t least = key_tile == 32 ? (getenv("PQ_L") ? atoi(getenv("PQ_L")) : 64) : (getenv("PQ_M") ? atoi(getenv("PQ_M")) : 512);
-    const int64_t most = ((int64_t)n_max + least - 1) / least;
-    p.splits = (int)(want < most ? want : most);
-    if (p.splits < 1) p.splits = 1;
+    // Splitting the keys fills the chip where row tiles are few, but the partial sums go through memory and the
+    // join is a launch: the number of splits with the least estimated time, in us.
+    const double tile_us = key_tile == 32 ? 7.0 : 2.2, key_tiles = (double)((n_max + key_tile - 1) / key_tile);
+    const int64_t room = p.waves == 8 ? 256 : 512;
+    double best = 0.0;
+    for (int s = 1; s <= 128 && s <= key_tiles; ++s) {
+        const double turns = (double)((busy * H * s + room - 1) / room), longest = (double)(int64_t)((key_tiles + s - 1) / s);
+        double us = turns * longest * tile_us;
+        if (s > 1) us += 8.0 + (double)(T * H * G) * (0.0008 + s * 0.00034);
+        if (s == 1 || us < best) {
+            best = us;
+            p.splits = s;
+        }
+    }
     const size_t rows = (size_t)T * H * G;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
@@ -812,9 +886,16 @@ template <int DT, bool GENERAL, int WAVES>
 int launch_prompt(const PromptArgs &a, hipStream_t stream) {
     auto kern = prompt_attend_kernel<DT, GENERAL, WAVES>;
     const size_t lds = PromptShape<WAVES>::kLds + 2 * (size_t)a.mask_words * 4;
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    static std::atomic<uint64_t> raised{0};              // devices on which the kernel's LDS limit is raised already
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    const uint64_t bit = 1ull << (device & 63);
+    if (e == hipSuccess && (device > 63 || !(raised.load(std::memory_order_relaxed) & bit))) {
+        e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        if (e == hipSuccess) raised.fetch_or(bit, std::memory_order_relaxed);
+    }
     if (e != hipSuccess) {
-        set_error("prompt_attend: cannot raise the LDS limit to %zu: %s", lds, hipGetErrorString(e));
+        set_error("prompt_attend: cannot raise the LDS limit: %s", hipGetErrorString(e));
         return PQHSA_ELAUNCH;
     }
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.H * a.tiles * a.splits)), dim3(WAVES * kWave), lds, stream, a);
@@ -901,7 +982,7 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
     }
     if (mass && n_max > 0) {
         a.mass_in = mass->in; a.mass_out = mass->out; a.mass_stride = mass->stride; a.decay = mass->decay; a.mass_rows = mass->rows;
-        const int keys = kMassWaves * 32;
+        const int keys = kMassWaves * mass_keys(kv->dtype);
         const dim3 grid((unsigned)((n_max + keys - 1) / keys), (unsigned)(B * H));
         PQHSA_DISPATCH_DTYPE(kv->dtype, hipLaunchKernelGGL(prompt_mass_kernel<DT>, grid, dim3(kMassWaves * kWave), 0, stream, a));
         rc = check_launch("prompt_mass");

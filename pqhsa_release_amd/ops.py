@@ -33,7 +33,7 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -904,8 +904,11 @@ class DenseAttendCall:
                       None if self._mass is None else ctypes.byref(self._mass), self._ws.data_ptr(), need)
 
     def run(self, stream: int | None = None) -> torch.Tensor:
-        with _on_device(self._device):
+        if torch.cuda.current_device() == self._device.index:
             rc = self._fn(*self._args, _stream() if stream is None else stream)
+        else:
+            with torch.cuda.device(self._device):
+                rc = self._fn(*self._args, _stream() if stream is None else stream)
         if rc:
             _lib.check(rc, "pqhsa_dense_attend_paged")
         return self.out
