@@ -473,8 +473,17 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 p[T][r] = exp2_fast(GENERAL ? s[T][r] - base : __builtin_fmaf(s[T][r], unit, -base));
-                l += p[T][r];
             }
+        // (a tile's weights among themselves first, in pairs: one after the other into l they would lose 1e-6 of it
+        // over a long walk, and every accumulated weight with it)
+        float sum[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[r] = kTT == 2 ? p[0][r] + p[kTT - 1][r] : p[0][r];
+#pragma unroll
+        for (int half = 8; half > 0; half /= 2)
+#pragma unroll
+            for (int r = 0; r < half; ++r) sum[r] += sum[r + half];
+        l += sum[0];
 #pragma unroll
         for (int u = 0; u < kSteps; ++u) {
             if constexpr (kF32) {
