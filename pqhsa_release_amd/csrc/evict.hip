@@ -77,6 +77,20 @@ __device__ inline void load_chunk(const float *mass, int j0, int len, float (&w)
     }
 }
 
+// whether any of this wave's keys lies below `len` (a chunk's last waves may have none: every instruction a key
+// costs is one of 16 waves' on one compute unit, so these leave early)
+__device__ inline bool wave_has_keys(int j0, int len) { return __builtin_amdgcn_readfirstlane(chunk_key(j0, 0) & ~63) < len; }
+
+// sum of the waves' numbers: of those in front of this one, of all
+__device__ inline uint32_t waves_before(const EvictLds &l) {
+    const int lane = threadIdx.x & 63;
+    return wave_total_u32(lane < (int)(threadIdx.x / kWave) ? l.wave_sums[lane] : 0u);
+}
+__device__ inline uint32_t waves_total(const EvictLds &l) {
+    const int lane = threadIdx.x & 63;
+    return wave_total_u32(lane < kEvictThreads / kWave ? l.wave_sums[lane] : 0u);
+}
+
 __device__ inline void clear_copies(EvictLds &l) {
 #pragma unroll
     for (int c = 0; c < kEvictCopies; ++c) l.copies[c][threadIdx.x] = make_uint2(0u, 0u);
@@ -86,6 +100,7 @@ __device__ inline void clear_copies(EvictLds &l) {
 __device__ inline void count_digits(EvictLds &l, const float (&w)[kEvictLoads], int j0, const EvictStream &s, int pass, uint32_t prefix) {
     uint32_t *copy = reinterpret_cast<uint32_t *>(l.copies[threadIdx.x & (kEvictCopies - 1)]);
     const int shift = digit_shift(pass), above = shift + digit_bits(pass);
+    if (!wave_has_keys(j0, s.high)) return;
 #pragma unroll
     for (int e = 0; e < kEvictLoads; ++e) {
         const int j = chunk_key(j0, e);
@@ -118,8 +133,7 @@ __device__ inline void find_cut(EvictLds &l, uint2 mine, uint32_t want) {
     uint32_t upto = wave_prefix_u32(both);
     if (lane == 63) l.wave_sums[wave] = upto;
     __syncthreads();
-#pragma unroll
-    for (int v = 0; v < kEvictThreads / kWave; ++v) upto += v < wave ? l.wave_sums[v] : 0u;
+    upto += waves_before(l);
     const uint32_t before = upto - both;
     if (before < want && want <= upto) {
         const bool first = want <= before + mine.x;
@@ -135,10 +149,7 @@ __device__ inline uint32_t block_total(EvictLds &l, uint32_t v) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) l.wave_sums[threadIdx.x / kWave] = v;
     __syncthreads();
-    v = 0;
-#pragma unroll
-    for (int w = 0; w < kEvictThreads / kWave; ++w) v += l.wave_sums[w];
-    return v;
+    return waves_total(l);
 }
 
 // outputs that do not depend on the weights: the new length and what lies behind the kept keys
@@ -150,6 +161,11 @@ __device__ inline void write_rest(const EvictArgs &a, int bh, int b, int len) {
         for (int64_t r = left + (int)threadIdx.x; r < a.out_stride; r += kEvictThreads) a.mass_out[(int64_t)bh * a.out_stride + r] = 0.0f;
 }
 
+// bits of `mask` below this lane's
+__device__ inline uint32_t lanes_below(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+}
+
 // The kept keys of a chunk, in order, behind `sure` keys that stay whatever the ties do and `ties` keys of
 // exactly the cut's weight; the first `quota` ties of the stream stay.
 __device__ inline void write_kept(const EvictArgs &a, EvictLds &l, int bh, const EvictStream &s, const float (&w)[kEvictLoads], int j0,
@@ -157,28 +173,31 @@ __device__ inline void write_kept(const EvictArgs &a, EvictLds &l, int bh, const
     const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
     uint64_t sure[kEvictLoads], tie[kEvictLoads];        // a bit per lane
     uint32_t counts = 0;
+    const bool some = wave_has_keys(j0, s.len);
+    const uint32_t open = s.all ? 0u : (uint32_t)(s.high - s.low);     // keys [low, low + open) are judged by their weight
+    if (s.want == 0) cut = ~0u;                          // (none of them stays: no weight is above, and no tie counts)
+    if (some) {
 #pragma unroll
-    for (int e = 0; e < kEvictLoads; ++e) {
-        const int j = chunk_key(j0, e);
-        const uint32_t k = order_key(w[e]);
-        const bool in = j < s.len, fixed = s.all || j < s.low || j >= s.high;
-        sure[e] = __ballot(in && (fixed || (s.want > 0 && k > cut)));
-        tie[e] = __ballot(in && !fixed && s.want > 0 && k == cut);
-        counts += (uint32_t)__popcll(sure[e]) | ((uint32_t)__popcll(tie[e]) << 16);
+        for (int e = 0; e < kEvictLoads; ++e) {
+            const int j = chunk_key(j0, e);
+            const uint32_t k = order_key(w[e]);
+            const bool judged = (uint32_t)(j - s.low) < open;
+            sure[e] = __ballot(j < s.len && (!judged || k > cut));
+            tie[e] = __ballot(judged && k == cut);
+            counts += (uint32_t)__popcll(sure[e]) | ((uint32_t)__popcll(tie[e]) << 16);
+        }
     }
     __syncthreads();
     if (lane == 0) l.wave_sums[wave] = counts;           // (at most 16 384 of each: no carry between the halves)
     __syncthreads();
-    uint32_t before = 0;
-#pragma unroll
-    for (int v = 0; v < kEvictThreads / kWave; ++v) before += v < wave ? l.wave_sums[v] : 0u;
+    if (!some) return;
+    const uint32_t before = waves_before(l);
     uint32_t n = sure_before + (before & 0xffffu), q = ties_before + (before >> 16);
-    const uint64_t below = (1ull << lane) - 1ull;
     int32_t *kept = a.kept + (int64_t)bh * a.keep;
     float *mass_out = a.mass_out ? a.mass_out + (int64_t)bh * a.out_stride : nullptr;
 #pragma unroll
     for (int e = 0; e < kEvictLoads; ++e) {
-        const uint32_t my_n = n + (uint32_t)__popcll(sure[e] & below), my_q = q + (uint32_t)__popcll(tie[e] & below);
+        const uint32_t my_n = n + lanes_below(sure[e]), my_q = q + lanes_below(tie[e]);
         if (((sure[e] >> lane) & 1) || (((tie[e] >> lane) & 1) && my_q < quota)) {
             const uint32_t r = my_n + min(my_q, quota);
             kept[r] = chunk_key(j0, e);
