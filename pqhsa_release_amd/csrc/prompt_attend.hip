@@ -358,18 +358,23 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     // Row r of K lies with its 16-byte piece c at place c ^ (r & 15); row r of V (2-byte types) at place
     // c ^ 2 (r & 7): the matrix operands' reads then spread over the banks.  A tile past the end is fetched
     // as zeros, so that the number of loads in flight is always the same.
-    auto fetch = [&](const char *base, int x, uint32_t to, bool values) {
+    // (All addresses are read before the first load is issued: no read of LDS may move past one, and a wait for each
+    // took half of the time that requesting a tile does.)
+    auto fetch = [&](int x) {
+        int64_t off[kLoads];
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int r = (wave * kLoads + i) * kPass + lane / kRowLanes;
-            const int turn = values ? (kF32 ? 0 : (r & 7) << 1) : r & 15;
-            const int64_t off = offs[(x & (kSlots - 1)) * 64 + r];
-            const char *p = off < 0 ? reinterpret_cast<const char *>(&g_zero_row) : base + off + ((lane % kRowLanes) ^ turn) * 16;
-            load_direct(lds0 + to + (wave * kLoads + i) * 1024, p);
-        }
+        for (int i = 0; i < kLoads; ++i) off[i] = offs[(x & (kSlots - 1)) * 64 + (wave * kLoads + i) * kPass + lane / kRowLanes];
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int r = (wave * kLoads + i) * kPass + lane / kRowLanes;
+                const int turn = v ? (kF32 ? 0 : (r & 7) << 1) : r & 15;
+                const char *p = (v ? a.kv.v_base : a.kv.k_base) + off[i] + ((lane % kRowLanes) ^ turn) * 16;
+                load_direct(lds0 + (v ? kVat : 0) + (x & (kStages - 1)) * kTileBytes + (wave * kLoads + i) * 1024,
+                            off[i] < 0 ? reinterpret_cast<const char *>(&g_zero_row) : p);
+            }
     };
-    auto fetch_keys = [&](int x) { fetch(a.kv.k_base, x, (x & (kStages - 1)) * kTileBytes, false); };
-    auto fetch_values = [&](int x) { fetch(a.kv.v_base, x, kVat + (x & (kStages - 1)) * kTileBytes, true); };
     // A weight of zero does not cancel an infinite or NaN value.  The walk is made without a thought for that;
     // where a sum then is not finite it is made again, with such values set aside in the tiles that some
     // rows of the workgroup do not see whole (they come back at the end, for the rows that see them).
@@ -548,10 +553,8 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
             if (wave < kSlots - 1) resolve(wave, reach);
             __syncthreads();
             if (docs && wave == 0) reach = tile_at(kSlots - 2);
-            fetch_keys(0);
-            fetch_values(0);
 #pragma unroll
-            for (int x = 1; x < kStages - 1; ++x) { fetch_keys(x); fetch_values(x); }
+            for (int x = 0; x < kStages - 1; ++x) fetch(x);
             direct_loads_done<kInFlight>();
             __syncthreads();
             if (careful && !all_see(t, wg_whole)) set_aside(lds + kVat);
@@ -562,8 +565,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
             const char *kl = lds + (x & (kStages - 1)) * kTileBytes;
             char *vl = lds + kVat + (x & (kStages - 1)) * kTileBytes;
             uint4 pw[kSteps];
-            fetch_keys(x + kStages - 1);
-            fetch_values(x + kStages - 1);
+            fetch(x + kStages - 1);
             score_product(kl, s);
             finish_scores(s, t, x & (kSlots - 1));
             raise_maximum(largest(s));
