@@ -436,6 +436,8 @@ int validate_score(const pqhsa_score *s, int n_max, const char *what) {
     PQHSA_REQUIRE(n_max <= 0x7fffffff - 65536, "%s: n_max %d is too large (key numbers are 32 bits)", what, n_max);
     PQHSA_REQUIRE(isfinite(s->scale), "%s: scale is not finite", what);
     PQHSA_REQUIRE(isfinite(s->softcap) && s->softcap >= 0.0f, "%s: softcap must be finite and not negative", what);
+    PQHSA_REQUIRE(isfinite(s->scale * kLog2e) && isfinite(s->softcap * kLog2e) && (s->softcap == 0.0f || isfinite(s->scale / s->softcap)),
+                  "%s: scale %g with softcap %g is out of range", what, s->scale, s->softcap);
     PQHSA_REQUIRE(s->window >= 0 && s->prefix >= 0, "%s: window %d and prefix %d must not be negative", what, s->window, s->prefix);
     PQHSA_REQUIRE(!s->docs || s->docs_stride >= n_max, "%s: docs_stride %lld below n_max %d", what, (long long)s->docs_stride, n_max);
     return PQHSA_OK;
@@ -519,7 +521,7 @@ extern "C" int pqhsa_dense_attend_paged(const void *q, int32_t q_dtype, int64_t 
     if (kv->paged)
         PQHSA_REQUIRE(blocks > 0 && (int64_t)kv->max_blocks * kv->block_size >= n_max,
                       "%s: %d blocks, and a table of %d x %d tokens for n_max %d", what, blocks, kv->max_blocks, kv->block_size, n_max);
-    PQHSA_REQUIRE((int64_t)B * H <= 0x7fffffff / kDenseRows, "%s: too many sequences and heads", what);
+    PQHSA_REQUIRE((int64_t)B * H <= (mass ? 65535 : 0x7fffffff / kDenseRows), "%s: too many sequences and heads", what);
     const DensePlan p = plan_dense(B, H, G, n_max, score, mass != nullptr);
     PQHSA_REQUIRE(p.splits <= 65535, "%s: n_max %d too large for one launch", what, n_max);
     if (workspace_bytes < p.bytes) {

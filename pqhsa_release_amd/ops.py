@@ -833,6 +833,18 @@ def _overlaps_itself(t: torch.Tensor) -> bool:
     return not (h >= HEAD_DIM and r >= (heads - 1) * h + HEAD_DIM or r >= HEAD_DIM and h >= (rows - 1) * r + HEAD_DIM)
 
 
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two ``[rows, heads, 128]`` tensors of one dtype may share memory (heads side by side in the rows
+    of one buffer do not)."""
+    size = a.element_size()
+    (ra, ha), (rb, hb) = _row_strides(a), _row_strides(b)
+    in_a, in_b = ((t.shape[1] - 1) * h + HEAD_DIM for t, h in ((a, ha), (b, hb)))
+    apart = (b.data_ptr() - a.data_ptr()) // size
+    if a.shape[0] == 0 or b.shape[0] == 0 or apart >= (a.shape[0] - 1) * ra + in_a or -apart >= (b.shape[0] - 1) * rb + in_b:
+        return False
+    return not (ra == rb > 0 and apart % ra >= in_a and apart % ra + in_b <= ra)
+
+
 def _check_seq_lens(seq_lens: torch.Tensor, batch: int) -> None:
     if seq_lens.dtype != torch.int32 or seq_lens.numel() != batch or not seq_lens.is_contiguous():
         raise ValueError(f"seq_lens must be a contiguous int32 [{batch}] tensor")
@@ -847,8 +859,11 @@ def _mass_struct(mass, mass_in, decay: float, rows: int, batch: int, heads: int,
         if t is not None and (t.dtype != torch.float32 or t.ndim != 3 or tuple(t.shape[:2]) != (batch, heads)
                               or t.shape[2] < n_max or not t.is_contiguous()):
             raise ValueError(f"mass must be a contiguous float32 [{batch}, {heads}, >= {n_max}] tensor")
-    if mass_in is not None and mass_in.shape != mass.shape:
-        raise ValueError("mass_in must have the shape of mass")
+    if mass_in is not None:
+        if mass_in.shape != mass.shape:
+            raise ValueError("mass_in must have the shape of mass")
+        if 0 < abs(mass_in.data_ptr() - mass.data_ptr()) < mass.numel() * 4:
+            raise ValueError("mass_in must be mass itself or lie apart from it")
     if not math.isfinite(float(decay)) or rows < 0:
         raise ValueError("decay must be finite, mass_rows not negative")
     m = _lib.Mass()
@@ -871,8 +886,9 @@ class DenseAttendCall:
     longer sequence is taken as having ``n_max`` tokens).  ``lse`` float32 ``[B, H*G]`` receives the
     log-sum-exp of every row.  ``mass`` float32 ``[B, H, >= n_max]`` receives ``decay * mass_in`` plus
     the weight the group's rows gave each key (``mass_in``: zeros when absent; may be ``mass``
-    itself).  The call owns its workspace, so calls that may overlap are different objects; a HIP
-    graph that holds ``run()`` keeps using it."""
+    itself, not a part of its memory).  ``out`` and ``q`` must not share memory.  The call owns its
+    workspace, so calls that may overlap are different objects; it, and every object a ``run(stream)``
+    on another stream or a HIP graph works on, has to outlive that work."""
 
     def __init__(self, q: torch.Tensor, out: torch.Tensor, kv: KvSource, groups: int, seq_lens: torch.Tensor, *,
                  n_max: int, rule: ScoreRule, lse: torch.Tensor | None = None, mass: torch.Tensor | None = None,
@@ -885,8 +901,8 @@ class DenseAttendCall:
         _check_rows(out, "out", h * groups, kv.dtype)
         if q.shape[0] != b or out.shape[0] != b:
             raise ValueError(f"q and out must have one row per sequence ({b})")
-        if _overlaps_itself(out):
-            raise ValueError("out: rows overlap in memory")
+        if _overlaps_itself(out) or _share_memory(q, out):
+            raise ValueError("out: rows overlap in memory, or with q's")
         _check_seq_lens(seq_lens, b)
         _check_bound(kv, n_max)
         rule.check(b, h * groups, n_max)
@@ -938,8 +954,8 @@ def prompt_attend(q: torch.Tensor, out: torch.Tensor, kv: KvSource, groups: int,
         raise ValueError(f"groups must be 1 to {MAX_GROUPS}")
     _check_rows(q, "q", h * groups, kv.dtype)
     _check_rows(out, "out", h * groups, kv.dtype)
-    if out.shape[0] != t or _overlaps_itself(out):
-        raise ValueError("out must have q's rows, none of which overlap in memory")
+    if out.shape[0] != t or _overlaps_itself(out) or _share_memory(q, out):
+        raise ValueError("out must have q's rows, none of which overlap in memory, nor with q's")
     if cu_rows.dtype != torch.int32 or tuple(cu_rows.shape) != (b + 1,) or not cu_rows.is_contiguous():
         raise ValueError(f"cu_rows must be a contiguous int32 [{b + 1}] tensor")
     _check_seq_lens(seq_lens, b)

@@ -190,3 +190,13 @@ def check_close(got, want, tol, what):
     bad = ~(off <= tol)
     assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} outside, worst {float((off / tol.clamp(min=1e-300))[bad].nan_to_num(1e9).max()):.3g} "
                            f"times the bound, first at {torch.nonzero(bad)[0].tolist()}: {got[bad][0]} for {want[bad][0]}")
+
+
+def far_away(source, blocks=140000):
+    """The pages of a 5-D cache moved to the far end of one whose K and V are more than 2^31 elements each."""
+    cache, table = source.keep
+    big = torch.empty(2, blocks, *cache.shape[2:], dtype=cache.dtype, device=cache.device)
+    assert big[0].numel() > 2 ** 31
+    first = blocks - cache.shape[1]
+    big[:, first:] = cache
+    return ops.kv_paged(big, table + first)

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from pqhsa_release_amd import _lib, ops
-from tests.dense_util import DIM, SCALE, DenseProblem, check_close
+from tests.dense_util import DIM, SCALE, DenseProblem, check_close, far_away
 
 gpu = pytest.mark.gpu
 BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
@@ -165,6 +165,28 @@ def test_visible_nan_and_infinite_scores_reach_the_output_of_their_row_only():
 
 
 @gpu
+def test_rows_beyond_32_bit_offsets():
+    p = DenseProblem([300, 77], [1, 1], heads=8, groups=4, layout="5d", block=16, seed=17)
+    near, q, sl, rule = p.source(), p.q.cuda(), p.seq_lens(), p.rule()
+    far = far_away(near)
+    outs = [torch.empty_like(q) for _ in range(2)]
+    for kv, out in zip((near, far), outs):
+        ops.dense_attend(q, out, kv, 4, sl, n_max=300, rule=rule)
+    assert torch.equal(*outs)
+
+
+@gpu
+def test_queries_and_outputs_side_by_side_in_one_buffer():
+    p = DenseProblem([90, 200, 33], [1, 1, 1], heads=2, groups=3, seed=18)
+    want, _, _, _ = run(p)
+    buffer = torch.full((3, 14, DIM), math.nan, dtype=p.dtype, device="cuda")
+    q, out = buffer[:, :6], buffer[:, 7:13]
+    q.copy_(p.q.cuda())
+    ops.dense_attend(q, out, p.source(), 3, p.seq_lens(), n_max=200, rule=p.rule())
+    assert torch.equal(out, want) and torch.equal(q, p.q.cuda()) and bool(buffer[:, 6].isnan().all()) and bool(buffer[:, 13].isnan().all())
+
+
+@gpu
 def test_refusals():
     p = DenseProblem([64, 30], [1, 1], heads=2, groups=2, seed=1)
     kv, rule, q, sl = p.source(), p.rule(), p.q.cuda(), p.seq_lens()
@@ -183,6 +205,11 @@ def test_refusals():
     refused("n_max", n_max=-1)
     refused("seq_lens", sl=sl.long())
     refused("overlap", out=out[:, :1].expand(-1, 4, -1))
+    refused("overlap", out=q)
+    both = torch.zeros(2, 7, DIM, dtype=p.dtype, device="cuda")
+    refused("overlap", q=both[:, :4], out=both[:, 3:])
+    weights = torch.zeros(3, 2, 64, device="cuda")
+    refused("apart", mass=weights[:2], mass_in=weights[1:])
     refused("aligned", q=torch.empty(2 * 4 * DIM + 1, dtype=p.dtype, device="cuda")[1:].view(2, 4, DIM))
     refused("mass", mass=torch.zeros(2, 2, 63, device="cuda"))
     refused("mass", mass=torch.zeros(2, 2, 64, device="cuda", dtype=torch.float64))
@@ -224,10 +251,12 @@ def test_c_entry_refuses_bad_arguments_before_any_gpu_work():
     assert call(n_max=1 << 20, ws_bytes=16) == -3 and b"workspace" in lib.pqhsa_last_error()
     mass.decay = 1.0
     assert call(mass=ctypes.byref(mass)) == -1
+    mass.out, mass.stride = 1 << 20, 10
+    assert call(B=70000, mass=ctypes.byref(mass), ws_bytes=1 << 60) == -1 and b"many" in lib.pqhsa_last_error()
     mass.out, mass.stride = 1 << 20, 9
     assert call(mass=ctypes.byref(mass)) == -1
     view.paged, view.block_table, view.block_size, view.max_blocks, view.stride_block = 1, 1 << 20, 16, 1, 2048
     assert call() == -1                      # a paged cache without blocks
     assert call(B=0) == 0
-    score.scale = math.nan
-    assert call() == -1
+    for score.scale, score.softcap in ((math.nan, 0.0), (3e38, 0.0), (1.0, 1e-39), (1.0, 3e38)):
+        assert call() == -1

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from pqhsa_release_amd import _lib, ops
-from tests.dense_util import DIM, SCALE, check_close
+from tests.dense_util import DIM, SCALE, check_close, far_away
 from tests.test_gpu_prompt import PromptProblem
 
 gpu = pytest.mark.gpu
@@ -194,6 +194,19 @@ def test_blocks_outside_either_cache():
     cache = src.keep[0].cpu()
     block = int(dst.keep[1][0, 0])
     assert torch.equal(cache[0, block, :, 0], K[0, 0, :16]) and torch.equal(cache[1, block, :, 0], V[0, 0, :16])
+
+
+@gpu
+def test_rows_beyond_32_bit_offsets():
+    src, K, V, dst, read = caches([500, 90], 8, BF, "5d", 16, 60, 6)
+    mass = torch.rand(2, 8, 500, generator=torch.Generator().manual_seed(1)).cuda()
+    sl = torch.tensor([500, 90], dtype=torch.int32, device="cuda")
+    near, _ = ops.evict(src, dst, mass, sl, keep=60, sink=1, recent=2, n_max=500)
+    far = far_away(src)
+    first = far.blocks - src.blocks
+    far_dst = ops.kv_paged(far.keep[0], dst.keep[1] + first)
+    kept, _ = ops.evict(far, far_dst, mass, sl, keep=60, sink=1, recent=2, n_max=500)
+    assert torch.equal(kept, near) and torch.equal(far.keep[0][:, first:], src.keep[0])
 
 
 @gpu
