@@ -59,6 +59,7 @@ __device__ inline void fold_stream_if_last(const AttendArgs &a, SharedLds &lds, 
     uint32_t *flags = a.arrive + (size_t)bh * G * kMaxSplits;
     if (tid == 0) __hip_atomic_store(flags + g * kMaxSplits + split, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     drain_memory_ops();  // ... and the flag is visible before the stream's flags are read
+    __syncthreads();     // (by any wave: one that read them before thread 0's store could miss a workgroup that misses this one)
     int missing = 0;
     for (int i = tid; i < G * splits; i += kAttThreads) {
         const int gs = i / splits, s = i % splits;
