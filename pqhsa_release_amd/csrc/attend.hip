@@ -144,7 +144,9 @@ int launch_attend(AttendArgs a, int q_dtype, int kv_dtype, int BH, int rows_max,
     const size_t lds = attend_lds_bytes(chunk);
     a.group_xcd = even_rows && (BH * a.splits) % 8 == 0;
     dim3 grid = a.group_xcd ? dim3(a.splits * a.G * BH) : dim3(a.splits, a.G, BH);
-    if (a.share_map && a.G >= 2 && a.G <= 8) {  // every selected row fetched once per KV head
+    // Every selected row fetched once per KV head.  (The fold takes a stream's partials two to a lane: streams cut
+    // into more of them than that fetch their rows one by one.)
+    if (a.share_map && a.G >= 2 && a.G <= 8 && (a.G + 1) * a.splits <= 2 * kWave) {
         const int SG = a.G <= 4 ? 4 : 8;
         const size_t lds_sh = SG == 4 ? attend_shared_lds_bytes<4>(chunk) : attend_shared_lds_bytes<8>(chunk);
 #define PQHSA_ATT_SH(KD, QD)                                                                                  \

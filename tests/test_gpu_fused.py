@@ -225,6 +225,20 @@ def test_rows_of_a_group_that_select_identical_disjoint_and_half_overlapping_key
         assert max(common) < 0.3
 
 
+@pytest.mark.parametrize("groups", [2, 7])
+def test_shared_fetch_of_one_stream_cut_into_many_chunks(groups):
+    """One stream takes 37 chunks per row of seven and 64 per row of two: more partials than the fold of a stream
+    keeps the weights of."""
+    dev = _cuda()
+    p = Problem(lens=[20000], heads=1, groups=groups, lists=32, dtype=torch.float32, seed=78)
+    idx = p.device_index(dev)
+    kv = _kv(p, "dense")
+    ws = ops.DecodeWorkspace(idx, p.G, ops.resolve_topk(p.n_max, 0.2, 0))
+    q = p.q_tensor().float()
+    shared, own = _steps(p, idx, kv, ws, q, 0.2, share_rows=True), _steps(p, idx, kv, ws, q, 0.2)
+    assert float((shared - own).abs().max()) <= 2e-5
+
+
 def test_shared_fetch_over_many_rows_and_chunks():
     """Many streams, the largest number of chunks per row the launch uses, rows that share most of their
     keys: every output row must be folded exactly once (rows start as NaN), over repeated steps."""
