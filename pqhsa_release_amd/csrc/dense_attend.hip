@@ -408,20 +408,40 @@ __global__ __launch_bounds__(256) void dense_mass_kernel(MassArgs a) {
         if (lane == 0) row[g] = l == 0.0f ? make_float2(INFINITY, 0.0f) : make_float2(top, 1.0f / l);   // +inf: the row gives no weight
     }
     __syncthreads();
+    // four keys a thread: 16-byte loads of every row's scores, several rows in flight
     const float *scores = a.scores + (int64_t)bh * a.G * a.score_stride;
+    const int64_t at = (int64_t)bh * a.stride;
+    const int j = j0 + 4 * tid;
+    if (j >= len) return;
+    float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto add = [&](float &to, float z, float2 r) {       // (-inf: masked, also from a row of NaN)
+        to += z == -INFINITY ? 0.0f : exp2_fast(z - r.x) * r.y;
+    };
+    if (a.in) {
 #pragma unroll
-    for (int i = 0; i < kMassKeys / 256; ++i) {
-        const int j = j0 + i * 256 + tid;
-        if (j >= len) break;
-        float w = a.in ? a.decay * a.in[(int64_t)bh * a.stride + j] : 0.0f;
-        const int v = j < range.first ? j : j - range.gap;
-        if (j < range.first || v >= range.first)
-            for (int g = 0; g < a.G; ++g) {
-                const float z = scores[g * a.score_stride + v];
-                w += z == -INFINITY ? 0.0f : exp2_fast(z - row[g].x) * row[g].y;   // (-inf: masked, also from a row of NaN)
-            }
-        a.out[(int64_t)bh * a.stride + j] = w;
+        for (int e = 0; e < 4; ++e)
+            if (j + e < len) w[e] = a.decay * a.in[at + j + e];
     }
+    const bool front = j + 3 < range.first, behind = j - range.gap >= range.first && (range.gap & 3) == 0;
+    if (j + 3 < len && (front || behind)) {
+        const float *p = scores + (front ? j : j - range.gap);
+#pragma unroll 4
+        for (int g = 0; g < a.G; ++g) {
+            const float4 z = *reinterpret_cast<const float4 *>(p + g * a.score_stride);
+            const float2 r = row[g];
+            add(w[0], z.x, r); add(w[1], z.y, r); add(w[2], z.z, r); add(w[3], z.w, r);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int v = j + e < range.first ? j + e : j + e - range.gap;
+            if (j + e < len && (j + e < range.first || v >= range.first))
+                for (int g = 0; g < a.G; ++g) add(w[e], scores[g * a.score_stride + v], row[g]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (j + e < len) a.out[at + j + e] = w[e];
 }
 
 // ---- host side ---------------------------------------------------------------------------
