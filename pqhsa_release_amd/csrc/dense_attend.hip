@@ -175,17 +175,25 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_attend_kernel(DenseArg
                 }
             }
         }
+        // (one branch a rule, not one a key)
         float z[kPer];
         bool live[kPer];
         float top = -INFINITY;
+        if (a.score.capped) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) z[e] = a.score.cap2 * tanh_score(s[e >> 2][e & 3] * a.score.in_cap);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) z[e] = s[e >> 2][e & 3] * a.score.scale2;
+        }
+        if (a.score.slopes) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) z[e] -= slope2 * (float)(len - 1 - range.key(v0 + at + kg * kPer + e));
+        }
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
-            const int v = at + kg * kPer + e;
-            live[e] = offs[v] >= 0;
-            float x = s[e >> 2][e & 3];
-            x = a.score.capped ? a.score.cap2 * tanh_score(x * a.score.in_cap) : x * a.score.scale2;
-            x -= slope2 * (float)(len - 1 - range.key(v0 + v));
-            z[e] = live[e] ? x : -INFINITY;
+            live[e] = offs[at + kg * kPer + e] >= 0;
+            z[e] = live[e] ? z[e] : -INFINITY;
             top = fmaxf(top, z[e]);
         }
         if (a.scores && n < a.G) {

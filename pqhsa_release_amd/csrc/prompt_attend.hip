@@ -425,16 +425,24 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     // the score rule on them: cap and bias (GENERAL), and the mask where the wave does not see the tile whole
     auto finish_scores = [&](f32x16 (&s)[kTT], int t, int slot) {
         const int k0 = key_tile(t);
-        if constexpr (GENERAL) {
+        if constexpr (GENERAL) {                         // (one branch a rule, not one a key)
+            if (a.score.capped) {
 #pragma unroll
-            for (int T = 0; T < kTT; ++T)
+                for (int T = 0; T < kTT; ++T)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int j = k0 + T * 32 + 8 * (r / 4) + 4 * kg + r % 4;
-                    const float x = s[T][r];
-                    s[T][r] = (a.score.capped ? a.score.cap2 * tanh_score(x * a.score.in_cap) : x * a.score.scale2)
-                              - slope2 * (float)abs(pos - j);
-                }
+                    for (int r = 0; r < 16; ++r) s[T][r] = a.score.cap2 * tanh_score(s[T][r] * a.score.in_cap);
+            } else {
+#pragma unroll
+                for (int T = 0; T < kTT; ++T)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[T][r] *= a.score.scale2;
+            }
+            if (a.score.slopes) {
+#pragma unroll
+                for (int T = 0; T < kTT; ++T)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[T][r] -= slope2 * (float)abs(pos - (k0 + T * 32 + 8 * (r / 4) + 4 * kg + r % 4));
+            }
         }
         const uint64_t exist = uniform(valid[slot]);
         if (all_see(t, wave_whole) && exist == (KT == 64 ? ~0ull : 0xffffffffull)) return;
