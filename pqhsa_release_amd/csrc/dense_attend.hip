@@ -19,6 +19,10 @@
 // The weights enter the second product as the sum of two 2-byte numbers (the rounded weight and its
 // rounded remainder), because a second product costs nothing here: the value sums are then as exact as
 // in fp32.
+//
+// Measured (bf16, 16-token pages): 4 x 131 072 tokens of 8 KV heads 392 us, 5.5 TB/s; 1 x 32 768 30 us, 26 of them
+// the attention at 5.1 TB/s and 4 the join; 16 x 700 12 us, which are two launches and the chain
+// length -> block -> row -> partial -> output, not bytes.
 #include "dense_common.h"
 
 namespace pqhsa {
@@ -377,9 +381,11 @@ int launch_join(const JoinArgs &a, int dtype, int64_t rows, hipStream_t stream) 
 }
 
 // ---- accumulated weight of every key -----------------------------------------------------
-// The group's rows have their (m, l) per split and the scores of all enumerated keys in memory: a
-// workgroup folds the statistics once and turns 1024 keys' scores into weights.  No atomics: a key has
-// one owner, which adds the G rows in order.
+// The group's rows have their (m, l) per split and the scores of all enumerated keys in memory (4 bytes each
+// against the 512 of a key's K and V; a second product would read K again): a workgroup folds the
+// statistics once and turns 1024 keys' scores into weights.  No atomics: a key has one owner, which adds the
+// G rows in order.  16 sequences of 16 384 to 65 536 keys, 4 x 7 heads: 26 us, and 60 us more in the attention for
+// writing the scores.
 struct MassArgs {
     const float *scores;
     int64_t score_stride;

@@ -12,6 +12,10 @@
 //
 // The move reads and writes 2 * 256 bytes (2-byte types) per kept key and is nearly all the traffic there
 // is: 16 bytes a lane, 16 lanes a row, all rows of a thread requested before the first is stored.
+//
+// Measured (bf16): 16 sequences of 16 384 to 65 536 keys, 8 heads, 8 192 kept each: the move 212 us, 5.0 TB/s read and
+// written (a large copy reaches 4.9); the selection 58 us in four launches.  One sequence of 8 192 keys, 8
+// heads, 4 096 kept: 12 + 6.5 us, the selection bound by the instructions of 8 workgroups on 8 compute units.
 #include "common.h"
 #include "dense_common.h"
 
