@@ -406,6 +406,7 @@ extern "C" int pqhsa_evict(const pqhsa_kv_view *src, int32_t src_blocks, const p
     PQHSA_REQUIRE(src->dtype == dst->dtype, "%s: caches of dtype %d and %d", what, src->dtype, dst->dtype);
     PQHSA_REQUIRE(B >= 0 && H > 0 && (int64_t)B * H <= 65535, "%s: B %d, H %d", what, B, H);
     PQHSA_REQUIRE(n_max >= 0 && mass_stride >= n_max, "%s: n_max %d, weights of stride %lld", what, n_max, (long long)mass_stride);
+    PQHSA_REQUIRE(n_max <= 0x7fffffff - 65536, "%s: n_max %d is too large (key numbers are 32 bits)", what, n_max);
     PQHSA_REQUIRE(sink >= 0 && recent >= 0 && keep > 0 && (int64_t)sink + recent <= keep, "%s: keep %d must be positive and hold sink %d + recent %d",
                   what, keep, sink, recent);
     const int left = keep < n_max ? keep : n_max;

@@ -92,9 +92,9 @@ __device__ inline void find_row_tile(const PromptArgs &a, int want, int &b_out, 
         const int upto = (int)wave_prefix_u32((uint32_t)tiles);
         const uint64_t hit = __ballot(before + upto > want);
         if (hit) {
-            const int who = __ffsll((unsigned long long)hit) - 1;
-            b_out = base + who;
-            tile_out = want - before - (__shfl(upto, who, kWave) - __shfl(tiles, who, kWave));
+            const int who = __ffsll((unsigned long long)hit) - 1, its = __shfl(tiles, who, kWave);
+            tile_out = want - before - (__shfl(upto, who, kWave) - its);
+            b_out = tile_out >= 0 && tile_out < its ? base + who : -1;   // (none: cu_rows that do not ascend)
             return;
         }
         before += __shfl(upto, 63, kWave);

@@ -183,6 +183,23 @@ def test_prompt_steps_eviction_and_further_steps_as_a_server_runs_them():
 
 
 @gpu
+@pytest.mark.parametrize("layouts", [("4d", "dense"), ("dense", "5d")])
+def test_from_one_layout_into_another(layouts):
+    lens, keep = [130, 40, 1], 48
+    src, K, V, _, _ = caches(lens, 2, BF, layouts[0], 16, keep, 11)
+    _, _, _, dst, read = caches(lens, 2, BF, layouts[1], 16, keep, 11)
+    mass = torch.rand(3, 2, 130, generator=torch.Generator().manual_seed(2))
+    kept, new = ops.evict(src, dst, mass.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), keep=keep, sink=2, recent=5, n_max=130)
+    assert new.tolist() == [48, 40, 1]
+    for b, n in enumerate(lens):
+        for h in range(2):
+            want = plain(mass[b, h].numpy(), n, keep, 2, 5)
+            assert np.array_equal(kept[b, h, : len(want)].cpu().numpy(), want) and bool((kept[b, h, len(want) :] == -1).all())
+            k, v = (ops.paged_gather_range(dst, b, 0, len(want))[i][h].cpu() for i in range(2))
+            assert torch.equal(k, K[b, h, torch.from_numpy(want)]) and torch.equal(v, V[b, h, torch.from_numpy(want)])
+
+
+@gpu
 def test_blocks_outside_either_cache():
     src, K, V, dst, read = caches([64], 1, BF, "5d", 16, 32, 5)
     src.keep[1][0, 1] = -1
@@ -278,6 +295,7 @@ def test_c_entry_refuses_bad_arguments_before_any_gpu_work():
     assert call(keep=2**31 - 1, sink=2**31 - 1, recent=2**31 - 1) == -1
     assert call(stride=9) == -1 and call(n_max=-1) == -1 and call(H=0) == -1 and call(B=70000) == -1 and call(mass=None) == -1
     assert call(out=1 << 20, out_stride=4) == -1 and call(ws=None) == -1 and call(ws=16) == -1
+    assert call(n_max=2**31 - 1, stride=1 << 31, ws_bytes=1 << 60) == -1 and b"large" in lib.pqhsa_last_error()
     assert call(n_max=1 << 20, stride=1 << 20, ws_bytes=256) == -3 and b"workspace" in lib.pqhsa_last_error()
     assert call(B=0) == 0
     dst.dtype = _lib.F16

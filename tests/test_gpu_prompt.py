@@ -204,6 +204,24 @@ def test_same_results_without_lse_and_from_a_replayed_graph():
 
 
 @gpu
+def test_no_keys_at_all_and_row_bounds_out_of_order():
+    p = PromptProblem([40, 40], [30, 30], heads=2, groups=2, seed=8)
+    kv, rule, q = p.source(), p.rule(), p.q.cuda()
+    out, lse = torch.full_like(q, 7.0), torch.full((60, 4), 7.0, device="cuda")
+    empty = torch.zeros(2, dtype=torch.int32, device="cuda")
+    ops.prompt_attend(q, out, kv, 2, p.cu_rows(), empty, n_max=0, rule=rule, lse=lse)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    one = torch.full_like(q[:2], 7.0)
+    ops.dense_attend(q[:2], one, kv, 2, empty, n_max=0, rule=rule)
+    assert bool((one == 0).all())
+    # bounds that do not ascend and run past the rows: rows of q only, nothing else is written
+    wild = torch.tensor([50, -3, 1 << 30], dtype=torch.int32, device="cuda")
+    out.fill_(7.0)
+    ops.prompt_attend(q, out, kv, 2, wild, p.seq_lens(), n_max=40, rule=rule)
+    assert bool(out.isfinite().all())
+
+
+@gpu
 def test_rows_beyond_32_bit_offsets():
     p = PromptProblem([300, 77], [90, 77], heads=8, groups=4, layout="5d", block=16, seed=17)
     near, q, sl, rule = p.source(), p.q.cuda(), p.seq_lens(), p.rule()
