@@ -78,29 +78,36 @@ __device__ inline PromptRows sequence_rows(const int32_t *cu, int64_t T, int b) 
     return {lo, (int)(hi - lo)};
 }
 
-// The workgroup's row tile: sequence and tile number inside it (b < 0: none).  Every wave finds it by itself.
+// The workgroup's row tile: its sequence (b < 0: none) with rows, length and prefix, and the tile's number in
+// it.  Every wave finds it by itself; a lane reads all of a sequence's numbers at once.
+struct RowTile {
+    int b, tile, first, rows, len, prefix;               // (T, and so the first row, is below 2^31)
+};
 template <int ROWS>
-__device__ inline void find_row_tile(const PromptArgs &a, int want, int &b_out, int &tile_out) {
+__device__ inline RowTile find_row_tile(const PromptArgs &a, int want) {
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int base = 0; base < a.B; base += 64) {
-        int tiles = 0;
+        int tiles = 0, len = 0, prefix = 0;
+        PromptRows r = {0, 0};
         if (base + lane < a.B) {
-            const PromptRows r = sequence_rows(a.cu_rows, a.T, base + lane);
+            r = sequence_rows(a.cu_rows, a.T, base + lane);
+            len = sequence_length(a.seq_lens, base + lane, a.n_max);
+            prefix = min(sequence_prefix(a.score, base + lane), len);
             tiles = (int)(((int64_t)r.rows * a.G + ROWS - 1) / ROWS);
         }
         const int upto = (int)wave_prefix_u32((uint32_t)tiles);
         const uint64_t hit = __ballot(before + upto > want);
         if (hit) {
-            const int who = __ffsll((unsigned long long)hit) - 1, its = __shfl(tiles, who, kWave);
-            tile_out = want - before - (__shfl(upto, who, kWave) - its);
-            b_out = tile_out >= 0 && tile_out < its ? base + who : -1;   // (none: cu_rows that do not ascend)
-            return;
+            const int who = __ffsll((unsigned long long)hit) - 1;
+            auto its = [&](int x) { return __builtin_amdgcn_readlane(x, who); };
+            RowTile t = {base + who, want - before - (its(upto) - its(tiles)), its((int)r.first), its(r.rows), its(len), its(prefix)};
+            if (t.tile < 0 || t.tile >= its(tiles)) t.b = -1;          // (cu_rows that do not ascend)
+            return t;
         }
-        before += __shfl(upto, 63, kWave);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
-    b_out = -1;
-    tile_out = 0;
+    return RowTile{-1, 0, 0, 0, 0, 0};
 }
 
 // w's two halves (one fp32 number) with infinite and NaN ones set to zero
@@ -197,15 +204,9 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
         order = blockIdx.x / streams;
     }
     const int h = stream % a.H, split = stream / a.H;
-    int b, tile;
-    find_row_tile<kPromptRows>(a, a.tiles - 1 - order, b, tile);      // the longest rows of a prompt first
-    if (b < 0) return;
-    b = __builtin_amdgcn_readfirstlane(b);
-    tile = __builtin_amdgcn_readfirstlane(tile);
-    PromptRows rows = sequence_rows(a.cu_rows, a.T, b);
-    rows.first = __builtin_amdgcn_readfirstlane((int)rows.first);    // (T is below 2^31)
-    rows.rows = __builtin_amdgcn_readfirstlane(rows.rows);
-    const int len = __builtin_amdgcn_readfirstlane(sequence_length(a.seq_lens, b, a.n_max));
+    const RowTile rows = find_row_tile<kPromptRows>(a, a.tiles - 1 - order);       // the longest rows of a prompt first
+    if (rows.b < 0) return;
+    const int b = rows.b, tile = rows.tile, len = rows.len;
     const int first_pos = len - rows.rows;
     const int64_t packed = (int64_t)rows.rows * a.G;
     const int64_t pr = (int64_t)tile * kPromptRows + wave * 32 + n;
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     const int prc = (int)(mine ? pr : packed - 1);       // rows past the end repeat the last one
     const int token = prc / a.G, g = prc - token * a.G;
     const int pos = first_pos + token;
-    const int prefix_all = __builtin_amdgcn_readfirstlane(min(sequence_prefix(a.score, b), len));
+    const int prefix_all = rows.prefix;
     // positions of the workgroup's rows, and of the wave's
     const int wg_lo = first_pos + (int)((int64_t)tile * kPromptRows / a.G);
     const int wg_hi = first_pos + (int)((min((int64_t)(tile + 1) * kPromptRows, packed) - 1) / a.G);
@@ -236,7 +237,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     // query rows as the second operand: lane (n, kg) holds row n
     u32x4 qf[kSlices];
     {
-        const char *p = a.q + ((rows.first + token) * a.q_row + (int64_t)(h * a.G + g) * a.q_head) * a.kv.esize;
+        const char *p = a.q + ((int64_t)(rows.first + token) * a.q_row + (int64_t)(h * a.G + g) * a.q_head) * a.kv.esize;
 #pragma unroll
         for (int u = 0; u < kSlices; ++u) qf[u] = *reinterpret_cast<const u32x4 *>(p + (u * 2 + kg) * 16);
     }
@@ -630,7 +631,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
         }
     }
     if (!mine) return;
-    const int64_t r = (rows.first + token) * (int64_t)(a.H * a.G) + h * a.G + g;
+    const int64_t r = (int64_t)(rows.first + token) * (a.H * a.G) + h * a.G + g;
     if (a.splits > 1) {
         if (kg == 0) a.part_ml[r * a.splits + split] = make_float2(m, l);
         if (l != 0.0f) {
@@ -647,7 +648,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     if (kg == 0 && a.lse) a.lse[r] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
     if (kg == 0 && a.row_ml) a.row_ml[r] = make_float2(m, l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    char *o = a.out + ((rows.first + token) * a.out_row + (int64_t)(h * a.G + g) * a.out_head) * a.kv.esize;
+    char *o = a.out + ((int64_t)(rows.first + token) * a.out_row + (int64_t)(h * a.G + g) * a.out_head) * a.kv.esize;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
