@@ -65,7 +65,8 @@ __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // tanh to fp32 accuracy relative to the result: the odd Taylor polynomial to x^13 below 0.45 (next term
 // 0.0015 x^15, under 2e-8 of the result there), (1 - e) / (1 + e) with e = exp(-2 |x|) <= 0.41 above.
 // inf gives 1, NaN stays NaN.
-__device__ inline float tanh_score(float x) {
+constexpr float kTanhSmall = 0.45f;
+__device__ inline float tanh_small(float x) {
     const float y = x * x;
     float p = 21844.0f / 6081075.0f;
     p = fmaf(p, y, -1382.0f / 155925.0f);
@@ -73,10 +74,12 @@ __device__ inline float tanh_score(float x) {
     p = fmaf(p, y, -17.0f / 315.0f);
     p = fmaf(p, y, 2.0f / 15.0f);
     p = fmaf(p, y, -1.0f / 3.0f);
-    p = fmaf(p * y, x, x);
+    return fmaf(p * y, x, x);
+}
+__device__ inline float tanh_score(float x) {
     const float e = exp2_fast(-2.0f * kLog2e * fabsf(x));
     const float big = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
-    return fabsf(x) < 0.45f ? p : copysignf(big, x);
+    return fabsf(x) < kTanhSmall ? tanh_small(x) : copysignf(big, x);
 }
 
 __device__ inline int sequence_length(const int32_t *seq_lens, int b, int n_max) {

@@ -164,11 +164,13 @@ __device__ uint4 g_zero_row;           // what lanes of a row that does not exis
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v lds_short4v;
 
-template <int DT, bool GENERAL, int WAVES>
+// RULE: 0 scores as they are (the scale goes into the exponent), 1 scaled, with a distance bias, 2 capped as well.  (One
+// kernel for 1 and 2: 99 instead of 93 us for 2 048 rows with a bias.)
+template <int DT, int RULE, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_attend_kernel(PromptArgs a) {
     using Shape = PromptShape<WAVES>;
     constexpr int kStages = Shape::kStages, kSlots = Shape::kSlots, kPromptRows = Shape::kRows, kThreads = Shape::kThreads;
-    constexpr bool kF32 = DT == PQHSA_F32;
+    constexpr bool kF32 = DT == PQHSA_F32, GENERAL = RULE > 0;
     constexpr int KT = kF32 ? 32 : 64;                   // keys per tile
     constexpr int kTT = KT / 32;                         // matrix tiles of keys
     constexpr int kRowBytes = kD * (kF32 ? 4 : 2);
@@ -431,12 +433,27 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     // the score rule on them: cap and bias (GENERAL), and the mask where the wave does not see the tile whole
     auto finish_scores = [&](f32x16 (&s)[kTT], int t, int slot) {
         const int k0 = key_tile(t);
-        if constexpr (GENERAL) {                         // (one branch a rule, not one a key)
-            if (a.score.capped) {
+        if constexpr (GENERAL) {
+            if constexpr (RULE == 2) {
+                float most = 0.0f;
 #pragma unroll
                 for (int T = 0; T < kTT; ++T)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[T][r] = a.score.cap2 * tanh_score(s[T][r] * a.score.in_cap);
+                    for (int r = 0; r < 16; ++r) {
+                        s[T][r] *= a.score.in_cap;
+                        most = fmaxf(most, fabsf(s[T][r]));
+                    }
+                if (__ballot(most >= kTanhSmall) == 0) {         // scores far below the cap: no exponential, no quotient
+#pragma unroll
+                    for (int T = 0; T < kTT; ++T)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[T][r] = a.score.cap2 * tanh_small(s[T][r]);
+                } else {
+#pragma unroll
+                    for (int T = 0; T < kTT; ++T)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[T][r] = a.score.cap2 * tanh_score(s[T][r]);
+                }
             } else {
 #pragma unroll
                 for (int T = 0; T < kTT; ++T)
@@ -911,9 +928,9 @@ PromptPlan plan_prompt(int64_t T, int B, int H, int G, int n_max, int rows_hint,
     return p;
 }
 
-template <int DT, bool GENERAL, int WAVES>
+template <int DT, int RULE, int WAVES>
 int launch_prompt(const PromptArgs &a, hipStream_t stream) {
-    auto kern = prompt_attend_kernel<DT, GENERAL, WAVES>;
+    auto kern = prompt_attend_kernel<DT, RULE, WAVES>;
     const size_t lds = PromptShape<WAVES>::kLds + 2 * (size_t)a.mask_words * 4;
     static std::atomic<uint64_t> raised{0};              // devices on which the kernel's LDS limit is raised already
     int device = 0;
@@ -929,6 +946,11 @@ int launch_prompt(const PromptArgs &a, hipStream_t stream) {
     }
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.H * a.tiles * a.splits)), dim3(WAVES * kWave), lds, stream, a);
     return check_launch("prompt_attend");
+}
+
+template <int DT, int WAVES>
+int launch_rule(int rule, const PromptArgs &a, hipStream_t stream) {
+    return rule == 2 ? launch_prompt<DT, 2, WAVES>(a, stream) : rule == 1 ? launch_prompt<DT, 1, WAVES>(a, stream) : launch_prompt<DT, 0, WAVES>(a, stream);
 }
 
 }  // namespace
@@ -998,10 +1020,8 @@ extern "C" int pqhsa_prompt_attend_paged(const void *q, int32_t q_dtype, int64_t
     a.row_ml = mass ? reinterpret_cast<float2 *>(w + p.row_at) : nullptr;
     PQHSA_REQUIRE(PromptShape<8>::kLds + 2 * (size_t)a.mask_words * 4 <= 160 * 1024, "%s: n_max %d too large for a document mask", what, n_max);
     if (T > 0) {
-        const bool general = score->softcap > 0.0f || score->slopes || !(score->scale > 0.0f);
-        PQHSA_DISPATCH_DTYPE(kv->dtype, 
-                              if (p.waves == 8) rc = general ? launch_prompt<DT, true, 8>(a, stream) : launch_prompt<DT, false, 8>(a, stream);
-                              else rc = general ? launch_prompt<DT, true, 4>(a, stream) : launch_prompt<DT, false, 4>(a, stream));
+        const int rule = score->softcap > 0.0f ? 2 : score->slopes || !(score->scale > 0.0f) ? 1 : 0;
+        PQHSA_DISPATCH_DTYPE(kv->dtype, rc = p.waves == 8 ? launch_rule<DT, 8>(rule, a, stream) : launch_rule<DT, 4>(rule, a, stream));
         if (rc) return rc;
         if (p.splits > 1) {
             JoinArgs j = {a.part_o, a.part_ml, p.splits, H * G, a.out, a.out_row, a.out_head, a.lse, a.row_ml, cu_rows + B};
