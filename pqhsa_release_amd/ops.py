@@ -7,6 +7,7 @@ the HIP kernels behind ``libpqhsa.so``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 
@@ -32,8 +33,11 @@ def dtype_code(dtype: torch.dtype) -> int:
     raise ValueError(f"unsupported dtype {dtype}")
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # current stream of a device, as an address (absent without a GPU build)
+
+
 def _stream() -> int:
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return _raw_stream(torch.cuda.current_device())
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -77,6 +81,17 @@ class KvSource:
 
     def ref(self):
         return ctypes.byref(self.view)
+
+    @functools.cached_property
+    def device_index(self) -> int:
+        indices = {t.get_device() for t in self.keep}
+        if len(indices) > 1:
+            raise ValueError("a cache and its block table on different devices")
+        return indices.pop()
+
+    @functools.cached_property
+    def storages(self) -> frozenset:
+        return frozenset(t.untyped_storage().data_ptr() for t in self.keep)
 
 
 def kv_contiguous(keys: torch.Tensor, values: torch.Tensor) -> KvSource:
@@ -769,7 +784,11 @@ class ScoreRule:
             s.docs, s.docs_stride = docs.data_ptr(), docs.stride(0) if docs.shape[0] > 1 else docs.shape[1]
         self.struct = s
         self.prefix, self.slopes, self.docs = prefix if isinstance(prefix, torch.Tensor) else None, slopes, docs
-        _need_cuda(*(t for t in (self.prefix, slopes, docs) if t is not None))
+        given = [t for t in (self.prefix, slopes, docs) if t is not None]
+        _need_cuda(*given)
+        if len({t.get_device() for t in given}) > 1:
+            raise ValueError("the tensors of a rule on different devices")
+        self.device_index = given[0].get_device() if given else None
 
     def ref(self):
         return ctypes.byref(self.struct)
@@ -783,20 +802,27 @@ class ScoreRule:
             raise ValueError(f"docs must be [{batch}, >= {n_max}]")
 
 
-def _one_device(first: torch.Tensor, *others) -> torch.device:
-    """The device all tensors of a call are on."""
-    _need_cuda(first)
+def _one_device(first: torch.Tensor, owners: tuple, *others) -> int:
+    """The device all tensors of a call are on, those of the caches and rules among ``owners`` included."""
+    index = first.get_device()
+    if index < 0:
+        _need_cuda(first)
+    for o in owners:
+        if o.device_index is not None and o.device_index != index:
+            raise ValueError(f"tensors on device {index} and {o.device_index} in one call")
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device} in one call")
-    return first.device
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"tensors on device {index} and {t.device} in one call")
+    return index
 
 
 class _on_device:
-    """Makes a tensor's device the current one for a call (nothing to do where it already is)."""
+    """Makes a device the current one for a call (nothing to do where it already is)."""
 
-    def __init__(self, device: torch.device) -> None:
-        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    __slots__ = ("_guard",)
+
+    def __init__(self, index: int) -> None:
+        self._guard = None if index == torch.cuda.current_device() else torch.cuda.device(index)
 
     def __enter__(self):
         if self._guard is not None:
@@ -807,23 +833,22 @@ class _on_device:
             self._guard.__exit__(*exc)
 
 
-def _check_rows(t: torch.Tensor, name: str, heads: int, dtype: torch.dtype) -> None:
-    vec = 16 // t.element_size()
-    if t.ndim != 3 or t.shape[1] != heads or t.shape[2] != HEAD_DIM or t.dtype != dtype:
-        raise ValueError(f"{name} must be [rows, {heads}, {HEAD_DIM}] of the cache's dtype {dtype}, got {tuple(t.shape)} {t.dtype}")
-    if (t.stride(2) != 1 or (t.shape[0] > 1 and t.stride(0) % vec) or (heads > 1 and t.stride(1) % vec)
-            or t.data_ptr() % 16):
+def _rows(t: torch.Tensor, name: str, heads: int, dtype: torch.dtype) -> tuple:
+    """(rows, heads, row stride, head stride, address) of a ``[rows, heads, 128]`` tensor, strides of what there is one of 0."""
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != HEAD_DIM or t.dtype != dtype:
+        raise ValueError(f"{name} must be [rows, {heads}, {HEAD_DIM}] of the cache's dtype {dtype}, got {tuple(shape)} {t.dtype}")
+    rows, (r, h, d), at = shape[0], t.stride(), t.data_ptr()
+    r, h = r if rows > 1 else 0, h if heads > 1 else 0
+    vec = 4 if dtype == torch.float32 else 8
+    if d != 1 or r % vec or h % vec or at % 16:
         raise ValueError(f"{name}: last dim contiguous, rows and heads 16-byte aligned")
+    return rows, heads, r, h, at
 
 
-def _row_strides(t: torch.Tensor) -> tuple:
-    return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
-
-
-def _overlaps_itself(t: torch.Tensor) -> bool:
-    """Whether two rows of a ``[rows, heads, 128]`` output could share memory (row stride >= heads, or the other way)."""
-    r, h = _row_strides(t)
-    rows, heads = t.shape[0], t.shape[1]
+def _overlaps_itself(out: tuple) -> bool:
+    """Whether two rows of an output could share memory (row stride >= heads, or the other way)."""
+    rows, heads, r, h, _ = out
     if rows <= 1 and heads <= 1:
         return False
     if rows <= 1:
@@ -833,16 +858,25 @@ def _overlaps_itself(t: torch.Tensor) -> bool:
     return not (h >= HEAD_DIM and r >= (heads - 1) * h + HEAD_DIM or r >= HEAD_DIM and h >= (rows - 1) * r + HEAD_DIM)
 
 
-def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two ``[rows, heads, 128]`` tensors of one dtype may share memory (heads side by side in the rows
-    of one buffer do not)."""
-    size = a.element_size()
-    (ra, ha), (rb, hb) = _row_strides(a), _row_strides(b)
-    in_a, in_b = ((t.shape[1] - 1) * h + HEAD_DIM for t, h in ((a, ha), (b, hb)))
-    apart = (b.data_ptr() - a.data_ptr()) // size
-    if a.shape[0] == 0 or b.shape[0] == 0 or apart >= (a.shape[0] - 1) * ra + in_a or -apart >= (b.shape[0] - 1) * rb + in_b:
+def _share_memory(a: tuple, b: tuple, size: int) -> bool:
+    """Whether two tensors of one dtype (``size`` bytes) may share memory (heads side by side in the rows of one
+    buffer do not)."""
+    rows_a, heads_a, ra, ha, at_a = a
+    rows_b, heads_b, rb, hb, at_b = b
+    in_a, in_b, apart = (heads_a - 1) * ha + HEAD_DIM, (heads_b - 1) * hb + HEAD_DIM, (at_b - at_a) // size
+    if rows_a == 0 or rows_b == 0 or apart >= (rows_a - 1) * ra + in_a or -apart >= (rows_b - 1) * rb + in_b:
         return False
     return not (ra == rb > 0 and apart % ra >= in_a and apart % ra + in_b <= ra)
+
+
+@functools.lru_cache(maxsize=1024)
+def _prompt_workspace(*sizes: int) -> int:
+    return _lib.load().pqhsa_prompt_attend_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _evict_workspace(*sizes: int) -> int:
+    return _lib.load().pqhsa_evict_workspace_bytes(*sizes)
 
 
 def _check_seq_lens(seq_lens: torch.Tensor, batch: int) -> None:
@@ -894,14 +928,13 @@ class DenseAttendCall:
                  n_max: int, rule: ScoreRule, lse: torch.Tensor | None = None, mass: torch.Tensor | None = None,
                  mass_in: torch.Tensor | None = None, decay: float = 1.0) -> None:
         b, h, n_max = kv.batch, kv.kv_heads, int(n_max)
-        device = _one_device(q, out, seq_lens, lse, mass, mass_in, *kv.keep, rule.prefix, rule.slopes, rule.docs)
+        device = _one_device(q, (kv, rule), out, seq_lens, lse, mass, mass_in)
         if not 1 <= groups <= MAX_GROUPS:
             raise ValueError(f"groups must be 1 to {MAX_GROUPS}")
-        _check_rows(q, "q", h * groups, kv.dtype)
-        _check_rows(out, "out", h * groups, kv.dtype)
-        if q.shape[0] != b or out.shape[0] != b:
+        rows, out_rows = _rows(q, "q", h * groups, kv.dtype), _rows(out, "out", h * groups, kv.dtype)
+        if rows[0] != b or out_rows[0] != b:
             raise ValueError(f"q and out must have one row per sequence ({b})")
-        if _overlaps_itself(out) or _share_memory(q, out):
+        if _overlaps_itself(out_rows) or _share_memory(rows, out_rows, q.element_size()):
             raise ValueError("out: rows overlap in memory, or with q's")
         _check_seq_lens(seq_lens, b)
         _check_bound(kv, n_max)
@@ -915,16 +948,13 @@ class DenseAttendCall:
             self._ws = torch.empty(need, dtype=torch.uint8, device=device)
         self._keep = (q, out, kv, seq_lens, rule, lse, mass, mass_in)
         self.out, self._device, self._fn = out, device, lib.pqhsa_dense_attend_paged
-        self._args = (q.data_ptr(), dtype_code(q.dtype), *_row_strides(q), out.data_ptr(), *_row_strides(out), kv.ref(),
-                      kv.blocks, b, h, groups, seq_lens.data_ptr(), n_max, rule.ref(), _ptr(lse),
+        self._args = (rows[4], dtype_code(q.dtype), *rows[2:4], out_rows[4], *out_rows[2:4], kv.ref(), kv.blocks,
+                      b, h, groups, seq_lens.data_ptr(), n_max, rule.ref(), _ptr(lse),
                       None if self._mass is None else ctypes.byref(self._mass), self._ws.data_ptr(), need)
 
     def run(self, stream: int | None = None) -> torch.Tensor:
-        if torch.cuda.current_device() == self._device.index:
-            rc = self._fn(*self._args, _stream() if stream is None else stream)
-        else:
-            with torch.cuda.device(self._device):
-                rc = self._fn(*self._args, _stream() if stream is None else stream)
+        with _on_device(self._device):
+            rc = self._fn(*self._args, _raw_stream(self._device) if stream is None else stream)
         if rc:
             _lib.check(rc, "pqhsa_dense_attend_paged")
         return self.out
@@ -949,12 +979,11 @@ def prompt_attend(q: torch.Tensor, out: torch.Tensor, kv: KvSource, groups: int,
     mass_in`` plus the weight that the last ``mass_rows`` rows of every sequence (0: all) gave each key.
     The other arguments are ``DenseAttendCall``'s; the workspace is a temporary of this call."""
     b, h, n_max, t = kv.batch, kv.kv_heads, int(n_max), q.shape[0]
-    device = _one_device(q, out, cu_rows, seq_lens, lse, mass, mass_in, *kv.keep, rule.prefix, rule.slopes, rule.docs)
+    device = _one_device(q, (kv, rule), out, cu_rows, seq_lens, lse, mass, mass_in)
     if not 1 <= groups <= MAX_GROUPS:
         raise ValueError(f"groups must be 1 to {MAX_GROUPS}")
-    _check_rows(q, "q", h * groups, kv.dtype)
-    _check_rows(out, "out", h * groups, kv.dtype)
-    if out.shape[0] != t or _overlaps_itself(out) or _share_memory(q, out):
+    rows, out_rows = _rows(q, "q", h * groups, kv.dtype), _rows(out, "out", h * groups, kv.dtype)
+    if out_rows[0] != t or _overlaps_itself(out_rows) or _share_memory(rows, out_rows, q.element_size()):
         raise ValueError("out must have q's rows, none of which overlap in memory, nor with q's")
     if cu_rows.dtype != torch.int32 or tuple(cu_rows.shape) != (b + 1,) or not cu_rows.is_contiguous():
         raise ValueError(f"cu_rows must be a contiguous int32 [{b + 1}] tensor")
@@ -964,15 +993,14 @@ def prompt_attend(q: torch.Tensor, out: torch.Tensor, kv: KvSource, groups: int,
     if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (t, h * groups) or not lse.is_contiguous()):
         raise ValueError(f"lse must be a contiguous float32 [{t}, {h * groups}] tensor")
     m = _mass_struct(mass, mass_in, decay, int(mass_rows), b, h, n_max)
-    lib = _lib.load()
-    rows_max = max(0, min(int(rows_max), t))
-    need = lib.pqhsa_prompt_attend_workspace_bytes(t, b, h, groups, n_max, rows_max, dtype_code(kv.dtype), int(mass is not None))
+    rows_max, code = max(0, min(int(rows_max), t)), dtype_code(kv.dtype)
+    need = _prompt_workspace(t, b, h, groups, n_max, rows_max, code, int(mass is not None))
     with _on_device(device):
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        rc = lib.pqhsa_prompt_attend_paged(q.data_ptr(), dtype_code(q.dtype), *_row_strides(q), out.data_ptr(),
-                                           *_row_strides(out), t, cu_rows.data_ptr(), kv.ref(), kv.blocks, b, h, groups,
-                                           seq_lens.data_ptr(), n_max, rows_max, rule.ref(), _ptr(lse),
-                                           None if m is None else ctypes.byref(m), ws.data_ptr(), need, _stream())
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        rc = _lib.load().pqhsa_prompt_attend_paged(rows[4], code, rows[2], rows[3], out_rows[4], out_rows[2], out_rows[3], t,
+                                                   cu_rows.data_ptr(), kv.ref(), kv.blocks, b, h, groups, seq_lens.data_ptr(),
+                                                   n_max, rows_max, rule.ref(), _ptr(lse), None if m is None else ctypes.byref(m),
+                                                   ws.data_ptr(), need, _raw_stream(device))
     _lib.check(rc, "pqhsa_prompt_attend_paged")
     return out
 
@@ -988,7 +1016,7 @@ def evict(kv: KvSource, dst: KvSource, mass: torch.Tensor, seq_lens: torch.Tenso
     last, and int32 ``[B]``.  ``mass_out`` float32 ``[B, H, >= min(keep, n_max)]`` receives the kept keys'
     weights, zeros behind them.  An index of the old cache does not describe the new one."""
     b, h, n_max, keep = kv.batch, kv.kv_heads, int(n_max), int(keep)
-    device = _one_device(mass, seq_lens, mass_out, *kv.keep, *dst.keep)
+    device = _one_device(mass, (kv, dst), seq_lens, mass_out)
     if dst.batch != b or dst.kv_heads != h or dst.dtype != kv.dtype:
         raise ValueError("dst must have the batch, KV heads and dtype of kv")
     if sink < 0 or recent < 0 or keep < 1 or sink + recent > keep:
@@ -997,8 +1025,7 @@ def evict(kv: KvSource, dst: KvSource, mass: torch.Tensor, seq_lens: torch.Tenso
     left = min(keep, n_max)
     if dst.capacity < left:
         raise ValueError(f"dst holds {dst.capacity} tokens per sequence, {left} may be kept")
-    shared = {t.untyped_storage().data_ptr() for t in kv.keep} & {t.untyped_storage().data_ptr() for t in dst.keep}
-    if shared and not (kv.view.paged and dst.view.paged and kv.view.block_table != dst.view.block_table):
+    if not kv.storages.isdisjoint(dst.storages) and not (kv.view.paged and dst.view.paged and kv.view.block_table != dst.view.block_table):
         raise ValueError("dst has to lie apart from kv: another cache, or a block table of its own")
     _check_seq_lens(seq_lens, b)
     if mass.dtype != torch.float32 or mass.ndim != 3 or tuple(mass.shape[:2]) != (b, h) or mass.shape[2] < n_max or not mass.is_contiguous():
@@ -1008,15 +1035,15 @@ def evict(kv: KvSource, dst: KvSource, mass: torch.Tensor, seq_lens: torch.Tenso
         raise ValueError(f"mass_out must be a contiguous float32 [{b}, {h}, >= {left}] tensor")
     if mass_out is not None and mass_out.untyped_storage().data_ptr() == mass.untyped_storage().data_ptr():
         raise ValueError("mass_out must not share memory with mass")
-    lib = _lib.load()
+    where, need = mass.device, _evict_workspace(b, h, n_max)
     with _on_device(device):
-        kept = torch.empty(b, h, keep, dtype=torch.int32, device=device)
-        new_lens = torch.empty(b, dtype=torch.int32, device=device)
-        need = lib.pqhsa_evict_workspace_bytes(b, h, n_max)
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        rc = lib.pqhsa_evict(kv.ref(), kv.blocks, dst.ref(), dst.blocks, b, h, mass.data_ptr(), mass.shape[2],
-                             seq_lens.data_ptr(), n_max, keep, int(sink), int(recent), kept.data_ptr(), new_lens.data_ptr(),
-                             _ptr(mass_out), 0 if mass_out is None else mass_out.shape[2], ws.data_ptr(), need, _stream())
+        kept = torch.empty(b, h, keep, dtype=torch.int32, device=where)
+        new_lens = torch.empty(b, dtype=torch.int32, device=where)
+        ws = torch.empty(need, dtype=torch.uint8, device=where)
+        rc = _lib.load().pqhsa_evict(kv.ref(), kv.blocks, dst.ref(), dst.blocks, b, h, mass.data_ptr(), mass.shape[2],
+                                     seq_lens.data_ptr(), n_max, keep, int(sink), int(recent), kept.data_ptr(), new_lens.data_ptr(),
+                                     _ptr(mass_out), 0 if mass_out is None else mass_out.shape[2], ws.data_ptr(), need,
+                                     _raw_stream(device))
     _lib.check(rc, "pqhsa_evict")
     return kept, new_lens
 
