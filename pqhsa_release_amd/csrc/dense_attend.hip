@@ -506,6 +506,9 @@ DensePlan plan_dense(int B, int H, int G, int n_max, const pqhsa_score *score, b
     // three rounds even that out (16 of 16384 to 65536 keys: 360 us, 381 in two).
     const int64_t want = B == 1 ? 512 : 1536;
     int64_t chunk = (streams * keys + want - 1) / want;
+    // No join where it costs more than walking on: two steps a wave (8 heads of 256 keys 8.9 us, 10.2 joined), and
+    // streams that fill the chip by themselves (512 of up to 512 keys 21.4 us, 25.4 joined; of up to 1024 33.9 and 34.8).
+    if (keys <= 256 || (streams >= 512 && keys <= 1024)) chunk = keys;
     chunk = (chunk + kDenseChunkMin - 1) / kDenseChunkMin * kDenseChunkMin;
     if (chunk > kDenseChunkMax) chunk = kDenseChunkMax;
     p.chunk = (int)chunk;
