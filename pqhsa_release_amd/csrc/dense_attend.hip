@@ -17,8 +17,8 @@
 //     read a whole row) and transposes the 8 x 8 block with byte permutes.
 //
 // The weights enter the second product as the sum of two 2-byte numbers (the rounded weight and its
-// rounded remainder), because a second product costs nothing here: the value sums are then as exact as
-// in fp32.
+// rounded remainder), because a second product costs nothing here: 2^-17 of a weight is rounded away at most in
+// bf16, 2^-22 in fp16 (there by a base near the step's own scores, and a remainder of its own scale).
 //
 // Measured (bf16, 16-token pages): 4 x 131 072 tokens of 8 KV heads 392 us, 5.5 TB/s; 1 x 32 768 30 us, 26 of them
 // the attention at 5.1 TB/s and 4 the join; 16 x 700 12 us, which are two launches and the chain
@@ -31,6 +31,10 @@ constexpr int kDenseThreads = 256;
 constexpr int kDenseWaves = kDenseThreads / kWave;
 constexpr int kDenseRows = 16;         // query rows of a matrix tile
 constexpr int kDenseChunkMin = 128, kDenseChunkMax = 4096;
+// fp16: the remainder enters times 2^11 (at most 2^14) and is summed by itself, so that a weight, at most 2^15, is off
+// by 2^-22 of itself or by 2^-36.  A step whose 32 keys all lie more than the drop (log2) below the base moves it:
+// otherwise its largest weight is 2^(13 - 22) at least, and 32 roundings of 2^-36 are 2^-22 of that.
+constexpr float kLowScale = 2048.0f, kDenseDrop = 22.0f;
 constexpr int kMassKeys = 1024;        // keys per workgroup of the weight accumulation
 
 struct DenseArgs {
@@ -146,10 +150,16 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_attend_kernel(DenseArg
         }
     };
 
-    float m = -INFINITY, l = 0.0f;
+    WeightBase<DT> base;
+    float l = 0.0f;
     f32x4 acc[8];                                        // dim (kg * 4 + r) * 8 + d of query row n in acc[d][r]
 #pragma unroll
     for (int d = 0; d < 8; ++d) acc[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 rem[base.kHalf ? 8 : 1];                       // fp16: sums of the scaled remainders
+    if constexpr (base.kHalf) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) rem[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
     if (wave * kStep < padded) request(wave * kStep);
     for (int at = wave * kStep; at < padded; at += kDenseWaves * kStep) {
@@ -208,21 +218,26 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_attend_kernel(DenseArg
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) p[t] = make_float4(z[4 * t], z[4 * t + 1], z[4 * t + 2], z[4 * t + 3]);
         }
-        if (__ballot(top > m + kMaxSlack)) {             // the row maximum moves: once or a few times per chunk
+        uint64_t low = __ballot(base.falls(top, kDenseDrop));
+        low &= low << 32 | low >> 32;                    // in all four lanes of a row
+        low &= low << 16 | low >> 48;
+        if (__ballot(base.raises(top)) | low) {          // a row's base moves: once or a few times per chunk
             top = fmaxf(top, __shfl_xor(top, 16, kWave));
             top = fmaxf(top, __shfl_xor(top, 32, kWave));
-            const float to = fmaxf(m, top);
-            const float f = m == to ? 1.0f : exp2_fast(m - to);
-            m = to;
+            const float f = base.move(top, kDenseDrop);
             l *= f;
 #pragma unroll
             for (int d = 0; d < 8; ++d) acc[d] *= f;
+            if constexpr (base.kHalf) {
+#pragma unroll
+                for (int d = 0; d < 8; ++d) rem[d] *= f;
+            }
         }
-        const float base = m == -INFINITY ? 0.0f : m;
+        const float origin = base.origin();
         float p[kPer];
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
-            p[e] = exp2_fast(z[e] - base);
+            p[e] = exp2_fast(z[e] - origin);
             l += p[e];
 #pragma unroll
             for (int w = 0; w < kVWords; ++w)
@@ -242,7 +257,8 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_attend_kernel(DenseArg
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 hw[w] = Half16<DT>::pack(p[2 * w], p[2 * w + 1]);
-                lw[w] = Half16<DT>::pack(p[2 * w] - Half16<DT>::low(hw[w]), p[2 * w + 1] - Half16<DT>::high(hw[w]));
+                const float x = p[2 * w] - Half16<DT>::low(hw[w]), y = p[2 * w + 1] - Half16<DT>::high(hw[w]);
+                lw[w] = base.kHalf ? Half16<DT>::pack(kLowScale * x, kLowScale * y) : Half16<DT>::pack(x, y);
             }
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
@@ -255,12 +271,19 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_attend_kernel(DenseArg
                 }
                 const uint4 vt = make_uint4(t[0], t[1], t[2], t[3]);
                 acc[d] = Half16<DT>::mfma16(vt, hi, acc[d]);
-                acc[d] = Half16<DT>::mfma16(vt, lo, acc[d]);
+                if constexpr (base.kHalf) rem[d] = Half16<DT>::mfma16(vt, lo, rem[d]);
+                else acc[d] = Half16<DT>::mfma16(vt, lo, acc[d]);
             }
         }
     }
     l += __shfl_xor(l, 16, kWave);
     l += __shfl_xor(l, 32, kWave);
+    const float settled = base.settle(l);
+    l *= settled;
+    if constexpr (base.kHalf) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[d] = (acc[d] + rem[d] * (1.0f / kLowScale)) * settled;
+    }
 
     // the four waves' results under the chunk's maximum
     __syncthreads();                                     // the address list is no longer read
@@ -268,7 +291,7 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_attend_kernel(DenseArg
     float *red_l = red_m + kDenseWaves * kDenseRows;
     float *red_o = red_l + kDenseWaves * kDenseRows;     // [waves][G][128]
     if (kg == 0) {
-        red_m[wave * kDenseRows + n] = m;
+        red_m[wave * kDenseRows + n] = base.m;
         red_l[wave * kDenseRows + n] = l;
     }
     if (n < a.G) {

@@ -19,10 +19,52 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// A running maximum is only moved (and what was summed under it rescaled) when a score passes it by
-// more than this, in log2 units: weights then stay below 2^8, which fp32 sums and 16-bit weights hold
-// without loss, and most tiles need no exchange between lanes at all.
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Weights are 2^(z2 - m) for a running base m, a former maximum, which is only moved (and what was summed
+// under it rescaled) when a score passes it by more than a slack, in log2 units: most tiles need no exchange
+// between lanes at all.  fp32 and bf16 hold such weights at any size.
 constexpr float kMaxSlack = 8.0f;
+// fp16 does not: below 2^-14 it has steps of 2^-24, whatever the size.  So its weights are 2^(z2 - m + 13), at most
+// 2^15, and the base also moves DOWN where all of a tile's scores for a row lie more than a drop (of the
+// kernel's) below it: keys far below the largest one, which only count together (those behind an attention
+// sink, say), then have the same bits.  It stays within 2^40 of the row's maximum: what is rounded away below that is
+// under 2^31 keys * 2^-78 * 2^16, less than fp16 outputs resolve.  Sums hold 2^15 * 2^40 * 2^16 * 2^31 keys.
+// This base is an integer, its moves exact.
+constexpr float kHalfSlack = 2.0f, kHalfShift = 13.0f, kHalfFall = 40.0f;
+template <int DT>
+struct WeightBase {
+    static constexpr bool kHalf = DT == PQHSA_F16;
+    static constexpr float kSlack = kHalf ? kHalfSlack : kMaxSlack;
+    float m = -INFINITY;                                 // the base; -inf: no visible key so far
+    float most = -INFINITY;                              // fp16: the row's maximum so far, rounded up
+    __device__ inline bool raises(float top) const { return top > m + kSlack; }
+    __device__ inline bool falls(float top, float drop) const { return kHalf && top < m - drop; }
+    // moves to a tile's maximum `top` of the row; returns what sums so far are multiplied by
+    __device__ inline float move(float top, float drop) {
+        float to = fmaxf(m, top), f;
+        if constexpr (kHalf) {
+            to = ceilf(to);
+            most = fmaxf(most, to);
+            if (falls(top, drop) && top > -INFINITY && m < INFINITY) to = fmaxf(ceilf(top), most - kHalfFall);
+            f = m == to ? 1.0f : __builtin_ldexpf(1.0f, (int)fmaxf(m - to, -200.0f));
+        } else {
+            f = m == to ? 1.0f : exp2_fast(m - to);
+        }
+        m = to;
+        return f;
+    }
+    // what exponents are taken relative to
+    __device__ inline float origin() const { return m == -INFINITY ? 0.0f : kHalf ? m - kHalfShift : m; }
+    // At the end: the base m to which a sum of weights belongs once it is multiplied by what this returns (fp16: brought
+    // to [1/2, 1), so that m + log2 of it, the log-sum-exp, is rounded once).
+    __device__ inline float settle(float sum) {
+        if constexpr (!kHalf) return 1.0f;
+        const int e = __builtin_amdgcn_frexp_expf(sum);  // (0 for zero, infinities and NaN)
+        m += (float)e - kHalfShift;
+        return __builtin_ldexpf(1.0f, -e);
+    }
+};
 
 // ---- score rule ---------------------------------------------------------------------
 // Scores are kept in units of log2: z2 = log2(e) * z, so that a weight is one exp2.
@@ -59,8 +101,6 @@ int validate_score(const pqhsa_score *s, int n_max, const char *what);
 int validate_mass(const pqhsa_mass *m, int n_max, const char *what);
 // host-side bound of the keys a row at the end of a sequence can see
 int64_t visible_bound(const pqhsa_score *s, int64_t n_max);
-
-__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // tanh to fp32 accuracy relative to the result.  Up to 1: x + x y p(y) with y = x^2, p the polynomial that meets
 // (tanh(x) / x - 1) / y at the seven Chebyshev points of y in [0, 1] (2e-8 of the result at most, 1.4 half steps

@@ -48,6 +48,20 @@ class DenseProblem:
         self.layout, self.block, self.cap = layout, block, cap
         self.gen, self.poison = g, poison
 
+    def set_levels(self, levels, *, spread=0.0, gain=1.0, silent=None):
+        """Every row scores key j of every sequence at about levels[j] nats (``spread``: standard deviation);
+        values are around ``gain``, and nothing for keys at levels above ``silent``."""
+        levels = torch.as_tensor(levels, dtype=torch.float32)
+        n = levels.numel()
+        self.q.zero_()
+        self.q[..., 0] = 8.0
+        self.K[:, :, :n, 0] = ((levels + spread * torch.randn(self.B, self.H, n, generator=self.gen)) / (8.0 * SCALE)).to(self.dtype)
+        V = gain * (1.0 + 0.25 * torch.randn(self.B, self.H, n, DIM, generator=self.gen))
+        if silent is not None:
+            V[:, :, levels > silent] = 0.0
+        self.V[:, :, :n] = V.to(self.dtype)
+        return self
+
     # ---- what a row sees, and the result in 64 bits
     def visible(self, b):
         """[rows, len] of sequence b."""

@@ -164,6 +164,36 @@ def test_visible_nan_and_infinite_scores_reach_the_output_of_their_row_only():
     assert bool(rest.isfinite().all())
 
 
+def sinks(n, every, drop):
+    """Levels of n keys: ``drop`` for one key in ``every``, 0 for the others."""
+    return [drop if j % every == 0 else 0.0 for j in range(n)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("spread", [0.0, 0.7])
+@pytest.mark.parametrize("drop", [10, 12, 14, 16, 18, 20, 24])
+def test_light_keys_behind_sinks_without_a_value(drop, spread, dtype):
+    """Keys whose weights are all far below the largest one make up the whole output, in values that
+    keep it above fp16's subnormal numbers."""
+    p = DenseProblem([4000, 90], [1, 1], heads=1, groups=2, dtype=dtype, seed=61)
+    check(p.set_levels(sinks(4000, 100, drop), spread=spread, gain=min(2e4, math.exp(drop) / 100), silent=5.0), mass=True)
+
+
+@gpu
+def test_light_keys_behind_a_sink_in_streams_of_one_chunk():
+    p = DenseProblem([1024] * 64, [1] * 64, heads=8, groups=1, dtype=HF, seed=62)
+    check(p.set_levels(sinks(1024, 1024, 14.0), spread=0.5, silent=5.0))
+
+
+@gpu
+def test_levels_of_keys_that_rise_and_fall_in_fp16():
+    g = torch.Generator().manual_seed(4)
+    levels = (torch.randint(0, 4, (200,), generator=g) * -6.0).repeat_interleave(20)
+    p = DenseProblem([4000, 1000], [1, 1], heads=2, groups=3, dtype=HF, seed=63)
+    check(p.set_levels(levels, spread=0.5, gain=2e4, silent=-16.0), mass=True)
+
+
 @gpu
 def test_rows_beyond_32_bit_offsets():
     p = DenseProblem([300, 77], [1, 1], heads=8, groups=4, layout="5d", block=16, seed=17)
