@@ -28,6 +28,9 @@
 namespace pqhsa {
 
 constexpr int kTileBytes = 16384;      // a K or V tile in LDS
+// fp16: a tile whose 64 keys all lie more than this (log2) below a row's base moves it.  Its largest weight is 2^(13 - 16)
+// at least otherwise, and 64 roundings of 2^-25 are 2^-16 of that.
+constexpr float kPromptDrop = 16.0f;
 
 // Two shapes of workgroup (32 rows a wave either way).
 template <int WAVES>
@@ -404,7 +407,8 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
         __syncthreads();
     };
 
-    float m, l;
+    WeightBase<DT> base;
+    float l;
     f32x16 acc[4];                                       // dim 32 dt + 8 (r / 4) + 4 kg + r % 4 of row n in acc[dt][r]
     // where GENERAL is false scores stay unscaled, the scale goes into the exponent
     const float unit = GENERAL ? 1.0f : a.score.scale2;
@@ -488,27 +492,29 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[T][r]);
         return top * unit;
     };
-    auto raise_maximum = [&](float top) {
-        if (__ballot(top > m + kMaxSlack)) {
+    auto move_base = [&](float top) {
+        uint64_t low = __ballot(base.falls(top, kPromptDrop));
+        low &= low << 32 | low >> 32;                    // in both lanes of a row
+        if (__ballot(base.raises(top)) | low) {
             top = fmaxf(top, __shfl_xor(top, 32, kWave));
-            const float to = fmaxf(m, top);
-            const float f = m == to ? 1.0f : exp2_fast(m - to);
-            m = to;
+            const float f = base.move(top, kPromptDrop);
             l *= f;
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt) acc[dt] *= f;
         }
     };
     // Weights, rounded to the value type for the product (their sum l is not): each at most half a step off,
-    // independently, no more than the output's own rounding.
+    // independently, no more than the output's own rounding.  (fp16 ones that lie more than 2^27 below the
+    // largest of their tile are subnormal: 2^-38 of that one off, at most.  A second product for the remainders, as
+    // in the single token's kernel, would cost half as many matrix instructions again.)
     auto weigh = [&](const f32x16 (&s)[kTT], uint4 (&pw)[kSteps]) {
-        const float base = m == -INFINITY ? 0.0f : m;
+        const float origin = base.origin();
         float p[kTT][16];
 #pragma unroll
         for (int T = 0; T < kTT; ++T)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                p[T][r] = exp2_fast(GENERAL ? s[T][r] - base : __builtin_fmaf(s[T][r], unit, -base));
+                p[T][r] = exp2_fast(GENERAL ? s[T][r] - origin : __builtin_fmaf(s[T][r], unit, -origin));
             }
         // (a tile's weights among themselves first, in pairs: one after the other into l they would lose 1e-6 of it
         // over a long walk, and every accumulated weight with it)
@@ -566,7 +572,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     const int t_first = next(t_begin);
 #pragma unroll 1
     for (bool careful = false;; careful = true) {
-        m = -INFINITY;
+        base = WeightBase<DT>();
         l = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt)
@@ -599,7 +605,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
             fetch(x + kStages - 1);
             score_product(kl, s);
             finish_scores(s, t, x & (kSlots - 1));
-            raise_maximum(largest(s));
+            move_base(largest(s));
             weigh(s, pw);
             value_product(lds0 + (uint32_t)(vl - lds), pw);
             if (wave == 0) {
@@ -646,6 +652,12 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
                     }
             }
         }
+    }
+    const float settled = base.settle(l), m = base.m;
+    l *= settled;
+    if constexpr (base.kHalf) {
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) acc[dt] *= settled;
     }
     if (!mine) return;
     const int64_t r = (int64_t)(rows.first + token) * (a.H * a.G) + h * a.G + g;

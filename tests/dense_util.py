@@ -121,6 +121,8 @@ class DenseProblem:
                     out[at : at + r, hq] = p @ V
                     tol[at : at + r, hq] = (HALF_STEP[self.dtype] * 1.001 * (p @ V).abs()
                                             + a * (2 * rel + n * U / 16 + low + self.weight_rounding()).reshape(-1, 1) + 2.0 ** -25)
+                    if n and self.weight_floor():
+                        tol[at : at + r, hq] += self.weight_floor() * p.amax(1, keepdim=True) * (see.double() @ V.abs())
                     lse[at : at + r, hq] = torch.where(alive, top.reshape(-1) + torch.log(l), torch.tensor(-math.inf, dtype=torch.float64))
                     lse_tol[at : at + r, hq] = dz + (n / 16 + 16) * U + 4 * U * lse[at : at + r, hq].abs().nan_to_num(posinf=0.0)
                     w_b[h, g], t_b[h, g] = p, 2 * rel + n * U / 16
@@ -132,6 +134,10 @@ class DenseProblem:
     def weight_rounding(self) -> float:
         """Relative rounding of the weights that enter the value product (one row per sequence: none
         beyond the remainder counted above)."""
+        return 0.0
+
+    def weight_floor(self) -> float:
+        """What a weight in the value product may be off, relative to the largest weight of its row."""
         return 0.0
 
     def mass(self, weights, weight_tol, last=0):

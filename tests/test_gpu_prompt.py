@@ -17,6 +17,11 @@ class PromptProblem(DenseProblem):
         # the 2-byte types round every weight once more, to half a step
         return 0.0 if self.dtype == FP else HALF_STEP[self.dtype]
 
+    def weight_floor(self):
+        # fp16 has no steps under 2^-24: a weight held as 2^(z2 - m + 13), m at most the maximum rounded up, is up to
+        # half of that off, 2^-25 2^-13 2^1 of the largest (keys of other tiles lose less)
+        return 2.0 ** -37 if self.dtype == HF else 0.0
+
     def cu_rows(self, device="cuda"):
         cu = [0]
         for r in self.rows:
@@ -139,6 +144,38 @@ def test_infinite_and_nan_values_reach_only_the_rows_that_see_them(dtype):
     assert bool(out[90:, 0, 7].isnan().all())
     assert bool((out[100, 0, 8] == math.inf).all()) and bool(out[101:, 0, 8].isnan().all())
     assert bool((out[100:, 0, 9] == math.inf).all()) and bool((out[101:, 0, 10] == -math.inf).all())
+
+
+def sinks(n, every, drop):
+    """Levels of n keys: ``drop`` for one key in ``every``, 0 for the others."""
+    return [drop if j % every == 0 else 0.0 for j in range(n)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("spread", [0.0, 0.7])
+@pytest.mark.parametrize("drop", [10, 12, 14, 16, 18, 20, 24])
+def test_light_keys_behind_sinks_without_a_value(drop, spread, dtype):
+    """Keys whose weights are all far below the largest one make up the whole output, in values that
+    keep it above fp16's subnormal numbers."""
+    p = PromptProblem([4000, 90], [5, 9], heads=1, groups=2, dtype=dtype, seed=61)
+    check(p.set_levels(sinks(4000, 100, drop), spread=spread, gain=min(2e4, math.exp(drop) / 100), silent=5.0), mass=2)
+
+
+@gpu
+@pytest.mark.parametrize("kw", [dict(), dict(docs=3), dict(softcap=40.0)])
+def test_levels_of_keys_that_rise_and_fall_in_fp16(kw):
+    g = torch.Generator().manual_seed(4)
+    levels = (torch.randint(0, 4, (50,), generator=g) * -6.0).repeat_interleave(20)
+    p = PromptProblem([1000, 700], [1000, 300], heads=2, groups=2, dtype=HF, seed=63, **kw)
+    check(p.set_levels(levels, spread=0.5, gain=2e4, silent=-16.0), mass=0)
+
+
+@gpu
+def test_light_keys_in_the_large_workgroups_in_fp16():
+    p = PromptProblem([901, 700, 512, 900, 650, 640, 577, 830], [512, 500, 512, 550, 520, 515, 490, 500], heads=2, groups=16,
+                      dtype=HF, seed=44)
+    check(p.set_levels(sinks(901, 150, 15.0), spread=0.5, gain=100.0, silent=5.0), mass=3)
 
 
 @gpu
