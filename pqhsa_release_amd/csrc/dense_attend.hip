@@ -151,129 +151,176 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_attend_kernel(DenseArg
     };
 
     WeightBase<DT> base;
-    float l = 0.0f;
+    float l;
     f32x4 acc[8];                                        // dim (kg * 4 + r) * 8 + d of query row n in acc[d][r]
-#pragma unroll
-    for (int d = 0; d < 8; ++d) acc[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     f32x4 rem[base.kHalf ? 8 : 1];                       // fp16: sums of the scaled remainders
-    if constexpr (base.kHalf) {
+    // A remainder of zero or below turns an infinite value into NaN, and so does a weight too small for its type.
+    // The walk is made without a thought for that; a wave whose sums are not all finite makes it again, with such
+    // values set aside and summed by themselves (all rows see the same keys, and no weight of theirs is nothing).
+    auto walk = [&](auto careful) {
+        constexpr bool CAREFUL = decltype(careful)::value;
+        base = WeightBase<DT>();
+        l = 0.0f;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) rem[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    if (wave * kStep < padded) request(wave * kStep);
-    for (int at = wave * kStep; at < padded; at += kDenseWaves * kStep) {
-        uint4 kc[kTiles][kSlices], vc[kPer][kVWords];
+        for (int d = 0; d < 8; ++d) acc[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (base.kHalf) {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-            for (int u = 0; u < kSlices; ++u) kc[t][u] = kf[t][u];
-#pragma unroll
-        for (int e = 0; e < kPer; ++e)
-#pragma unroll
-            for (int w = 0; w < kVWords; ++w) vc[e][w] = vf[e][w];
-        if (at + kDenseWaves * kStep < padded) request(at + kDenseWaves * kStep);
-
-        f32x4 s[kTiles];
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-            s[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int u = 0; u < kSlices; ++u) {
-                if constexpr (kF32) {
-                    const f32x4 x = __builtin_bit_cast(f32x4, kc[t][u]), y = __builtin_bit_cast(f32x4, qf[u]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[c], y[c], s[t], 0, 0, 0);
-                } else {
-                    s[t] = Half16<DT>::mfma16(kc[t][u], qf[u], s[t]);
-                }
-            }
+            for (int d = 0; d < 8; ++d) rem[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
         }
-        // (one branch a rule, not one a key)
-        float z[kPer];
-        bool live[kPer];
-        float top = -INFINITY;
-        if (a.score.capped) {
+        if (!CAREFUL && wave * kStep < padded) request(wave * kStep);
+        for (int at = wave * kStep; at < padded; at += kDenseWaves * kStep) {
+            uint4 kc[kTiles][kSlices], vc[kPer][kVWords];
+            if (CAREFUL) request(at);                    // (nothing in flight: a walk for few)
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) z[e] = a.score.cap2 * tanh_score(s[e >> 2][e & 3] * a.score.in_cap);
-        } else {
+            for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) z[e] = s[e >> 2][e & 3] * a.score.scale2;
-        }
-        if (a.score.slopes) {
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) z[e] -= slope2 * (float)(len - 1 - range.key(v0 + at + kg * kPer + e));
-        }
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            live[e] = offs[at + kg * kPer + e] >= 0;
-            z[e] = live[e] ? z[e] : -INFINITY;
-            top = fmaxf(top, z[e]);
-        }
-        if constexpr (SCORES) {
-            // Every lane stores, the ones that repeat row 0 what row 0's lane does: with a branch around them the
-            // compiler could not count the stores, and waited for them where it waits for the next step's rows
-            // (330 instead of 322 us in 16 sequences of 16 384 to 65 536 keys).
-            float4 *p = reinterpret_cast<float4 *>(a.scores + ((int64_t)bh * a.G + g) * a.score_stride + v0 + at + kg * kPer);
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) p[t] = make_float4(z[4 * t], z[4 * t + 1], z[4 * t + 2], z[4 * t + 3]);
-        }
-        uint64_t low = __ballot(base.falls(top, kDenseDrop));
-        low &= low << 32 | low >> 32;                    // in all four lanes of a row
-        low &= low << 16 | low >> 48;
-        if (__ballot(base.raises(top)) | low) {          // a row's base moves: once or a few times per chunk
-            top = fmaxf(top, __shfl_xor(top, 16, kWave));
-            top = fmaxf(top, __shfl_xor(top, 32, kWave));
-            const float f = base.move(top, kDenseDrop);
-            l *= f;
-#pragma unroll
-            for (int d = 0; d < 8; ++d) acc[d] *= f;
-            if constexpr (base.kHalf) {
-#pragma unroll
-                for (int d = 0; d < 8; ++d) rem[d] *= f;
-            }
-        }
-        const float origin = base.origin();
-        float p[kPer];
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            p[e] = exp2_fast(z[e] - origin);
-            l += p[e];
-#pragma unroll
-            for (int w = 0; w < kVWords; ++w)
-                if (!live[e]) vc[e][w] = make_uint4(0u, 0u, 0u, 0u);  // whatever lies there must not reach the product
-        }
-        if constexpr (kF32) {
+                for (int u = 0; u < kSlices; ++u) kc[t][u] = kf[t][u];
 #pragma unroll
             for (int e = 0; e < kPer; ++e)
 #pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    const f32x4 x = __builtin_bit_cast(f32x4, vc[e][d >> 2]);
-                    acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[d & 3], p[e], acc[d], 0, 0, 0);
-                }
-        } else {
-            uint4 hi, lo;
-            uint32_t *hw = reinterpret_cast<uint32_t *>(&hi), *lw = reinterpret_cast<uint32_t *>(&lo);
+                for (int w = 0; w < kVWords; ++w) vc[e][w] = vf[e][w];
+            if (!CAREFUL && at + kDenseWaves * kStep < padded) request(at + kDenseWaves * kStep);
+
+            f32x4 s[kTiles];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                hw[w] = Half16<DT>::pack(p[2 * w], p[2 * w + 1]);
-                const float x = p[2 * w] - Half16<DT>::low(hw[w]), y = p[2 * w + 1] - Half16<DT>::high(hw[w]);
-                lw[w] = base.kHalf ? Half16<DT>::pack(kLowScale * x, kLowScale * y) : Half16<DT>::pack(x, y);
+            for (int t = 0; t < kTiles; ++t) {
+                s[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int u = 0; u < kSlices; ++u) {
+                    if constexpr (kF32) {
+                        const f32x4 x = __builtin_bit_cast(f32x4, kc[t][u]), y = __builtin_bit_cast(f32x4, qf[u]);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[c], y[c], s[t], 0, 0, 0);
+                    } else {
+                        s[t] = Half16<DT>::mfma16(kc[t][u], qf[u], s[t]);
+                    }
+                }
+            }
+            // (one branch a rule, not one a key)
+            float z[kPer];
+            bool live[kPer];
+            float top = -INFINITY;
+            if (a.score.capped) {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) z[e] = a.score.cap2 * tanh_score(s[e >> 2][e & 3] * a.score.in_cap);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) z[e] = s[e >> 2][e & 3] * a.score.scale2;
+            }
+            if (a.score.slopes) {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) z[e] -= slope2 * (float)(len - 1 - range.key(v0 + at + kg * kPer + e));
             }
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                uint32_t t[4];
+            for (int e = 0; e < kPer; ++e) {
+                live[e] = offs[at + kg * kPer + e] >= 0;
+                z[e] = live[e] ? z[e] : -INFINITY;
+                top = fmaxf(top, z[e]);
+            }
+            if constexpr (SCORES) {
+                // Every lane stores, the ones that repeat row 0 what row 0's lane does: with a branch around them the
+                // compiler could not count the stores, and waited for them where it waits for the next step's rows
+                // (330 instead of 322 us in 16 sequences of 16 384 to 65 536 keys).
+                float4 *p = reinterpret_cast<float4 *>(a.scores + ((int64_t)bh * a.G + g) * a.score_stride + v0 + at + kg * kPer);
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) p[t] = make_float4(z[4 * t], z[4 * t + 1], z[4 * t + 2], z[4 * t + 3]);
+            }
+            uint64_t low = __ballot(base.falls(top, kDenseDrop));
+            low &= low << 32 | low >> 32;                    // in all four lanes of a row
+            low &= low << 16 | low >> 48;
+            if (__ballot(base.raises(top)) | low) {          // a row's base moves: once or a few times per chunk
+                top = fmaxf(top, __shfl_xor(top, 16, kWave));
+                top = fmaxf(top, __shfl_xor(top, 32, kWave));
+                const float f = base.move(top, kDenseDrop);
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < 8; ++d) acc[d] *= f;
+                if constexpr (base.kHalf) {
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) rem[d] *= f;
+                }
+            }
+            if constexpr (CAREFUL) {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e)
+#pragma unroll
+                    for (int w = 0; w < kVWords; ++w)
+                        vc[e][w] = make_uint4(finite_part<DT>(vc[e][w].x), finite_part<DT>(vc[e][w].y), finite_part<DT>(vc[e][w].z), finite_part<DT>(vc[e][w].w));
+            }
+            const float origin = base.origin();
+            float p[kPer];
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                p[e] = exp2_fast(z[e] - origin);
+                l += p[e];
+#pragma unroll
+                for (int w = 0; w < kVWords; ++w)
+                    if (!live[e]) vc[e][w] = make_uint4(0u, 0u, 0u, 0u);  // whatever lies there must not reach the product
+            }
+            if constexpr (kF32) {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e)
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) {
+                        const f32x4 x = __builtin_bit_cast(f32x4, vc[e][d >> 2]);
+                        acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[d & 3], p[e], acc[d], 0, 0, 0);
+                    }
+            } else {
+                uint4 hi, lo;
+                uint32_t *hw = reinterpret_cast<uint32_t *>(&hi), *lw = reinterpret_cast<uint32_t *>(&lo);
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const uint32_t x = reinterpret_cast<const uint32_t *>(&vc[2 * w][0])[d >> 1];
-                    const uint32_t y = reinterpret_cast<const uint32_t *>(&vc[2 * w + 1][0])[d >> 1];
-                    t[w] = __builtin_amdgcn_perm(y, x, d & 1 ? 0x07060302u : 0x05040100u);
+                    hw[w] = Half16<DT>::pack(p[2 * w], p[2 * w + 1]);
+                    const float x = p[2 * w] - Half16<DT>::low(hw[w]), y = p[2 * w + 1] - Half16<DT>::high(hw[w]);
+                    lw[w] = base.kHalf ? Half16<DT>::pack(kLowScale * x, kLowScale * y) : Half16<DT>::pack(x, y);
                 }
-                const uint4 vt = make_uint4(t[0], t[1], t[2], t[3]);
-                acc[d] = Half16<DT>::mfma16(vt, hi, acc[d]);
-                if constexpr (base.kHalf) rem[d] = Half16<DT>::mfma16(vt, lo, rem[d]);
-                else acc[d] = Half16<DT>::mfma16(vt, lo, acc[d]);
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    uint32_t t[4];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t x = reinterpret_cast<const uint32_t *>(&vc[2 * w][0])[d >> 1];
+                        const uint32_t y = reinterpret_cast<const uint32_t *>(&vc[2 * w + 1][0])[d >> 1];
+                        t[w] = __builtin_amdgcn_perm(y, x, d & 1 ? 0x07060302u : 0x05040100u);
+                    }
+                    const uint4 vt = make_uint4(t[0], t[1], t[2], t[3]);
+                    acc[d] = Half16<DT>::mfma16(vt, hi, acc[d]);
+                    if constexpr (base.kHalf) rem[d] = Half16<DT>::mfma16(vt, lo, rem[d]);
+                    else acc[d] = Half16<DT>::mfma16(vt, lo, acc[d]);
+                }
             }
+        }
+    };
+    walk(std::false_type{});
+    float zero[4] = {};                                  // NaN where a sum is not finite
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            zero[r] = __builtin_fmaf(acc[d][r], 0.0f, zero[r]);
+            if constexpr (base.kHalf) zero[r] = __builtin_fmaf(rem[d][r], 0.0f, zero[r]);
+        }
+    if (__builtin_expect(__ballot(zero[0] + zero[1] + (zero[2] + zero[3]) != 0.0f) != 0, 0)) {
+        walk(std::true_type{});
+        float odd[8] = {};                               // dims n * 8 + d of this lane's keys
+#pragma unroll 1
+        for (int at = wave * kStep; at < padded; at += kDenseWaves * kStep)
+#pragma unroll 1
+            for (int e = 0; e < kPer; ++e) {
+                const int64_t off = offs[at + kg * kPer + e];
+                if (off < 0) continue;
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    const float x = load1<DT>(a.kv.v_base + off, n * 8 + d);
+                    if (!(fabsf(x) < INFINITY)) odd[d] += x;
+                }
+            }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            odd[d] += __shfl_xor(odd[d], 16, kWave);
+            odd[d] += __shfl_xor(odd[d], 32, kWave);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[d][r] += __shfl(odd[d], kg * 4 + r, kWave);
         }
     }
     l += __shfl_xor(l, 16, kWave);
@@ -312,7 +359,7 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_attend_kernel(DenseArg
 #pragma unroll
         for (int w = 0; w < kDenseWaves; ++w) {
             const float mw = red_m[w * kDenseRows + g];
-            const float f = mw == top ? 1.0f : exp2_fast(mw - top);   // (a wave without a visible key holds zeros)
+            const float f = mw == top ? 1.0f : exp2_something(mw - top);   // (a wave without a visible key holds zeros)
             sum += f * red_l[w * kDenseRows + g];
             o += f * red_o[((size_t)w * a.G + g) * kD + d];
         }
@@ -360,7 +407,7 @@ __global__ __launch_bounds__(256) void dense_join_kernel(JoinArgs a) {
             if (s0 + i * kGroups >= a.splits) y[i] = make_float2(-INFINITY, 0.0f);
             top = fmaxf(top, y[i].x);
         }
-        const float back = m == top ? 1.0f : exp2_fast(m - top);
+        const float back = m == top ? 1.0f : exp2_something(m - top);
         m = top;
         l *= back;
         o.x *= back; o.y *= back; o.z *= back; o.w *= back;
@@ -368,7 +415,7 @@ __global__ __launch_bounds__(256) void dense_join_kernel(JoinArgs a) {
         for (int i = 0; i < kBatch; ++i) {
             // a split without a visible key wrote no sums: whatever lies there is not used
             const bool some = y[i].y != 0.0f;            // (NaN counts)
-            const float f = y[i].x == m ? 1.0f : exp2_fast(y[i].x - m);
+            const float f = y[i].x == m ? 1.0f : exp2_something(y[i].x - m);
             l += some ? f * y[i].y : 0.0f;
             o.x += some ? f * x[i].x : 0.0f;
             o.y += some ? f * x[i].y : 0.0f;
@@ -388,7 +435,7 @@ __global__ __launch_bounds__(256) void dense_join_kernel(JoinArgs a) {
         l = 0.0f;
 #pragma unroll
         for (int w = 0; w < kGroups; ++w) {
-            const float f = y[w].x == m ? 1.0f : exp2_fast(y[w].x - m);   // (a group without a visible key holds zeros)
+            const float f = y[w].x == m ? 1.0f : exp2_something(y[w].x - m);   // (a group without a visible key holds zeros)
             l += f * y[w].y;
             x += f * red[w][tid];
         }

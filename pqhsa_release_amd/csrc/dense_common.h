@@ -4,6 +4,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace pqhsa {
@@ -20,6 +22,8 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// never quite zero: an infinite partial sum stays one under any other base
+__device__ inline float exp2_something(float x) { return fmaxf(exp2_fast(x), 0x1p-149f); }
 
 // Weights are 2^(z2 - m) for a running base m, a former maximum, which is only moved (and what was summed
 // under it rescaled) when a score passes it by more than a slack, in log2 units: most tiles need no exchange
@@ -180,6 +184,17 @@ struct Half16<PQHSA_F16> {
     static __device__ inline float low(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[0]; }
     static __device__ inline float high(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[1]; }
 };
+
+// w's two halves (one fp32 number) with infinite and NaN ones set to zero
+template <int DT>
+__device__ inline uint32_t finite_part(uint32_t w) {
+    if constexpr (DT == PQHSA_F32) {
+        return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
+    } else {
+        constexpr uint32_t e = DT == PQHSA_BF16 ? 0x7f80u : 0x7c00u;
+        return ((w & e) == e ? 0u : w & 0xffffu) | ((w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u);
+    }
+}
 
 // ---- partial results of a split key range, and their join ---------------------------------
 // Row r (query row * heads + head) of split s: part_o[(r * splits + s) * 128 ..] the weighted value sum

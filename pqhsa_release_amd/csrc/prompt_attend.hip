@@ -113,17 +113,6 @@ __device__ inline RowTile find_row_tile(const PromptArgs &a, int want) {
     return RowTile{-1, 0, 0, 0, 0, 0};
 }
 
-// w's two halves (one fp32 number) with infinite and NaN ones set to zero
-template <int DT>
-__device__ inline uint32_t finite_part(uint32_t w) {
-    if constexpr (DT == PQHSA_F32) {
-        return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
-    } else {
-        constexpr uint32_t e = DT == PQHSA_BF16 ? 0x7f80u : 0x7c00u;
-        return ((w & e) == e ? 0u : w & 0xffffu) | ((w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u);
-    }
-}
-
 __device__ inline uint64_t uniform(uint64_t x) {         // the same in every lane
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32)) << 32;
 }

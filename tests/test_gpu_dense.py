@@ -195,6 +195,42 @@ def test_levels_of_keys_that_rise_and_fall_in_fp16():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("length", [200, 3000])
+def test_infinite_and_nan_values_reach_the_output_of_the_rows_that_see_them(dtype, length):
+    """As the definition has it: a positive weight times infinity, whatever the weight; elements without one stay exact."""
+    p = DenseProblem([length, 150], [1, 1], heads=2, groups=3, dtype=dtype, poison=False, seed=14)
+    want, want_lse, tol, lse_tol, _, _ = p.evaluate()
+    p.V[0, 0, 90, 7] = math.nan
+    p.V[0, 0, 100, 8] = math.inf
+    p.V[0, 0, 101, 8] = -math.inf
+    p.V[0, 0, 100, 9] = p.V[0, 0, length - 1, 9] = math.inf
+    p.V[0, 0, 101, 10] = -math.inf
+    p.V[0, 0, length - 1, 127] = math.inf
+    p.V[0, 0, length:] = math.inf                        # (behind the sequence: seen by nobody)
+    out, lse, _, _ = run(p)
+    check_close(lse, want_lse, lse_tol, "lse")
+    clean = torch.ones(2, 6, DIM, dtype=torch.bool)
+    clean[0, :3, 7:11] = clean[0, :3, 127] = False
+    check_close(out[clean.cuda()], want[clean], tol[clean], "out")
+    assert bool(out[0, :3, 7:9].isnan().all())
+    assert bool((out[0, :3, 9] == math.inf).all()) and bool((out[0, :3, 10] == -math.inf).all()) and bool((out[0, :3, 127] == math.inf).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+def test_an_infinite_value_of_a_key_with_next_to_no_weight(dtype):
+    """exp(-150) is no fp32 number, but it is more than nothing; in the sink's chunk, in another, in one wave's and another's keys."""
+    p = DenseProblem([1500, 200], [1, 1], heads=1, groups=2, dtype=dtype, poison=False, seed=15).set_levels([150.0] + [0.0] * 1499)
+    p.V[0, 0, 57, 3] = p.V[0, 0, 7, 4] = p.V[0, 0, 1400, 5] = math.inf
+    p.V[1, 0, 33, 6] = -math.inf
+    out, _, _, _ = run(p)
+    assert bool((out[0, :, 3:6] == math.inf).all()) and bool((out[1, :, 6] == -math.inf).all())
+    out[0, :, 3:6] = out[1, :, 6] = 0.0
+    assert bool(out.isfinite().all())
+
+
+@gpu
 def test_rows_beyond_32_bit_offsets():
     p = DenseProblem([300, 77], [1, 1], heads=8, groups=4, layout="5d", block=16, seed=17)
     near, q, sl, rule = p.source(), p.q.cuda(), p.seq_lens(), p.rule()
