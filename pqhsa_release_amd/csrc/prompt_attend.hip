@@ -40,7 +40,7 @@ struct PromptShape {
     static constexpr int kRows = WAVES * 32;             // packed rows
     static constexpr int kStages = WAVES / 2;            // K/V tiles in LDS
     static constexpr int kSlots = 2 * kStages;           // tiles whose row addresses are known or on their way
-    static constexpr int kLds = 2 * kStages * kTileBytes + kSlots * (64 * 8 + 64 * 4 + 64 * 4 + 8 + 4) + 16;
+    static constexpr int kLds = 2 * kStages * kTileBytes + kSlots * (64 * 8 + 64 * 4 + 64 * 4 + 8 + 4) + 16 + kD * 4;
 };
 
 struct PromptArgs {
@@ -178,8 +178,9 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     int32_t *kdoc = phys + kSlots * 64;                                            // [slots][64] documents
     uint64_t *valid = reinterpret_cast<uint64_t *>(kdoc + kSlots * 64);            // [slots] rows that exist
     int32_t *tiles = reinterpret_cast<int32_t *>(valid + kSlots);                  // [slots] tile of the walk (documents)
-    int32_t *poison = tiles + kSlots;                                              // [2]: a sum is not finite; values were set aside
-    uint32_t *wanted = reinterpret_cast<uint32_t *>(poison + 4);                   // [mask_words] tiles to walk
+    int32_t *poison = tiles + kSlots;                                              // [3]: a sum is not finite; values were set aside in tiles seen in part; in whole ones
+    uint32_t *odd = reinterpret_cast<uint32_t *>(poison + 4);                      // [128 dims] 1: inf, 2: -inf, 4: NaN among the latter
+    uint32_t *wanted = odd + kD;                                                   // [mask_words] tiles to walk
     uint32_t *pure = wanted + a.mask_words;                                        // [mask_words] tiles of the rows' one document
     const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char *)lds;
 
@@ -375,24 +376,34 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
                             off[i] < 0 ? reinterpret_cast<const char *>(&g_zero_row) : p);
             }
     };
-    // A weight of zero does not cancel an infinite or NaN value.  The walk is made without a thought for that;
-    // where a sum then is not finite it is made again, with such values set aside in the tiles that some
-    // rows of the workgroup do not see whole (they come back at the end, for the rows that see them).
-    auto set_aside = [&](char *vl) {
+    // A weight of zero does not cancel an infinite or NaN value, and one that is too small for its type loses it.  The
+    // walk is made without a thought for that; where a sum then is not finite it is made again with such values
+    // set aside.  They come back at the end: those of a tile that all rows of the workgroup see whole by the dim, the
+    // others for the rows that see them.
+    auto set_aside = [&](char *vl, bool whole) {
         bool bad = false;
 #pragma unroll
         for (int i = 0; i < kTileBytes / 16 / kThreads; ++i) {
-            u32x4 *p = reinterpret_cast<u32x4 *>(vl + (i * kThreads + tid) * 16);
+            const int at = i * kThreads + tid;
+            u32x4 *p = reinterpret_cast<u32x4 *>(vl + at * 16);
             const u32x4 x = *p;
             u32x4 y;
 #pragma unroll
             for (int w = 0; w < 4; ++w) y[w] = finite_part<DT>(x[w]);
-            if (x[0] != y[0] || x[1] != y[1] || x[2] != y[2] || x[3] != y[3]) {
-                *p = y;
-                bad = true;
+            if (x[0] == y[0] && x[1] == y[1] && x[2] == y[2] && x[3] == y[3]) continue;
+            *p = y;
+            bad = true;
+            if (!whole) continue;
+            const int row = at / kRowLanes, first = ((at % kRowLanes) ^ (kF32 ? 0 : (row & 7) << 1)) * (kD / kRowLanes);
+#pragma unroll
+            for (int e = 0; e < kD / kRowLanes; ++e) {
+                float v;
+                if constexpr (kF32) v = __uint_as_float(x[e]);
+                else v = e & 1 ? Half16<DT>::high(x[e / 2]) : Half16<DT>::low(x[e / 2]);
+                if (!(fabsf(v) < INFINITY)) atomicOr(odd + first + e, v > 0.0f ? 1u : v < 0.0f ? 2u : 4u);
             }
         }
-        if (bad) poison[1] = 1;
+        if (bad) poison[whole ? 2 : 1] = 1;
         __syncthreads();
     };
 
@@ -557,7 +568,8 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
     // arrived by the end of iteration x + stages - 2.  Tile x's own slot is still being read (its documents),
     // so the first that may be looked up anew is the one of tile x - 1.
     constexpr int kInFlight = (kStages - 2) * 2 * kLoads;
-    if (tid < 2) poison[tid] = 0;
+    if (tid < 3) poison[tid] = 0;
+    if (tid < kD) odd[tid] = 0u;
     const int t_first = next(t_begin);
 #pragma unroll 1
     for (bool careful = false;; careful = true) {
@@ -583,7 +595,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
             for (int x = 0; x < kStages - 1; ++x) fetch(x);
             direct_loads_done<kInFlight>();
             __syncthreads();
-            if (careful && !all_see(t, wg_whole)) set_aside(lds + kVat);
+            if (careful) set_aside(lds + kVat, all_see(t, wg_whole));
         }
 #pragma unroll 1
         for (int x = 0; t < t_end; ++x) {
@@ -605,7 +617,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
             if (t1 < t_end) {
                 direct_loads_done<kInFlight>();
                 __syncthreads();
-                if (careful && !all_see(t1, wg_whole)) set_aside(lds + kVat + ((x + 1) & (kStages - 1)) * kTileBytes);
+                if (careful) set_aside(lds + kVat + ((x + 1) & (kStages - 1)) * kTileBytes, all_see(t1, wg_whole));
             }
             t = t1;
         }
@@ -621,7 +633,16 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
         if (!poison[0]) break;
     }
     l += __shfl_xor(l, 32, kWave);
-    if (t_first < t_end && poison[1]) {                  // the infinities and NaN that were set aside
+    if (t_first < t_end && poison[2]) {                  // the infinities and NaN that were set aside
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const uint32_t x = odd[dt * 32 + 8 * (r / 4) + 4 * kg + r % 4];
+                if (x) acc[dt][r] += x == 1u ? INFINITY : x == 2u ? -INFINITY : NAN;
+            }
+    }
+    if (t_first < t_end && poison[1]) {
 #pragma unroll 1
         for (int t = t_first; t < t_end; t = next(t + 1)) {
             const int k0 = key_tile(t);

@@ -179,6 +179,38 @@ def test_light_keys_in_the_large_workgroups_in_fp16():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+def test_an_infinite_value_of_a_key_with_next_to_no_weight(dtype):
+    """exp(-150) is no fp32 number, but it is more than nothing: every row that sees the key, in tiles that all rows
+    see whole and others, is infinite there."""
+    p = PromptProblem([500, 1500], [500, 3], heads=1, groups=2, dtype=dtype, poison=False, seed=15).set_levels([150.0] + [0.0] * 1499)
+    p.V[0, 0, 57, 3] = p.V[0, 0, 7, 4] = math.inf
+    p.V[1, 0, 1400, 5] = p.V[1, 0, 20, 6] = -math.inf
+    p.V[1, 0, 21, 6] = math.inf
+    out, _, _, _ = run(p)
+    assert bool((out[57:500, :, 3] == math.inf).all()) and bool((out[7:500, :, 4] == math.inf).all())
+    assert bool((out[500:, :, 5] == -math.inf).all()) and bool(out[500:, :, 6].isnan().all())
+    out[57:500, :, 3] = out[7:500, :, 4] = out[500:, :, 5:7] = 0.0
+    assert bool(out.isfinite().all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+def test_infinite_values_in_the_large_workgroups(dtype):
+    """Sequence 0's rows are at positions 389 to 900: one value only some of them see, one that all see, in whole tiles."""
+    p = PromptProblem([901, 700, 512, 900, 650, 640, 577, 830], [512, 500, 512, 550, 520, 515, 490, 500], heads=2, groups=16,
+                      dtype=dtype, poison=False, seed=45)
+    want, _, tol, _, _, _ = p.evaluate()
+    p.V[0, 1, 600, 4], p.V[0, 1, 100, 5], p.V[0, 1, 620, 6] = math.inf, -math.inf, math.nan
+    out, _, _, _ = run(p)
+    clean = torch.ones(want.shape, dtype=torch.bool)
+    clean[600 - 389 : 512, 16:, 4] = clean[:512, 16:, 5] = clean[620 - 389 : 512, 16:, 6] = False
+    check_close(out[clean.cuda()], want[clean], tol[clean], "out")
+    assert bool((out[600 - 389 : 512, 16:, 4] == math.inf).all()) and bool((out[:512, 16:, 5] == -math.inf).all())
+    assert bool(out[620 - 389 : 512, 16:, 6].isnan().all())
+
+
+@gpu
 def test_block_table_entries_outside_the_cache_mask_their_keys():
     kw = dict(heads=2, groups=2, block=16, poison=False, seed=9)
     p, q = PromptProblem([160], [160], **kw), PromptProblem([160], [160], **kw)
