@@ -221,7 +221,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 8 ? 1 : 2) void prompt_atte
 
     // the walk: tiles [0, walk_a), then walk_b onwards, `count` in all
     const int end = max(0, min(len, wg_hi + 1));
-    const int begin = a.score.window > 0 ? max(0, wg_lo - window + 1) : 0;
+    const int begin = a.score.window > 0 ? max(0, max(wg_lo, 0) - window + 1) : 0;   // (rows in front of the sequence see nothing)
     const int walk_a = wg_hi >= 0 ? (prefix_all + KT - 1) / KT : 0;
     const int walk_b = max(begin / KT, walk_a);
     const int count = wg_hi >= 0 ? walk_a + max(0, (end + KT - 1) / KT - walk_b) : 0;

@@ -120,6 +120,13 @@ def test_rows_in_front_of_their_sequence_see_nothing():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("prefix", [None, 3])
+def test_a_window_near_2_31_with_rows_in_front_of_their_sequence(dtype, prefix):
+    check(PromptProblem([5, 70], [9, 90], heads=2, groups=2, dtype=dtype, seed=8, window=2**31 - 1, prefix=prefix), mass=0)
+
+
+@gpu
 def test_a_long_prompt_and_large_scores():
     check(PromptProblem([1700], [1700], heads=1, groups=2, dtype=BF, seed=5, q_gain=6.0))
 
