@@ -21,11 +21,12 @@ class DenseProblem:
     ``poison`` fills every place of the cache that no row may look at with NaN and infinities."""
 
     def __init__(self, lens, rows, *, heads=2, groups=4, dtype=torch.bfloat16, layout="5d", block=16, softcap=0.0,
-                 window=0, prefix=None, slopes=False, docs=0, poison=True, pad=0, seed=0, extra=5, q_gain=1.0):
+                 window=0, prefix=None, slopes=False, docs=0, poison=True, pad=0, seed=0, extra=5, q_gain=1.0,
+                 scale=SCALE):
         g = torch.Generator().manual_seed(seed)
         self.lens, self.rows, self.B, self.H, self.G = list(lens), list(rows), len(lens), heads, groups
         self.dtype, self.n_max = dtype, max([0, *lens])
-        self.softcap, self.window, self.pad = softcap, window, pad
+        self.softcap, self.window, self.pad, self.scale = softcap, window, pad, scale
         self.prefix = prefix
         self.slopes = torch.rand(heads * groups, generator=g) * 0.05 if slopes else None
         self.docs = None
@@ -55,7 +56,7 @@ class DenseProblem:
         n = levels.numel()
         self.q.zero_()
         self.q[..., 0] = 8.0
-        self.K[:, :, :n, 0] = ((levels + spread * torch.randn(self.B, self.H, n, generator=self.gen)) / (8.0 * SCALE)).to(self.dtype)
+        self.K[:, :, :n, 0] = ((levels + spread * torch.randn(self.B, self.H, n, generator=self.gen)) / (8.0 * self.scale)).to(self.dtype)
         V = gain * (1.0 + 0.25 * torch.randn(self.B, self.H, n, DIM, generator=self.gen))
         if silent is not None:
             V[:, :, levels > silent] = 0.0
@@ -98,9 +99,9 @@ class DenseProblem:
                 for g in range(self.G):
                     hq = h * self.G + g
                     q = self.q[at : at + r, hq].double()
-                    z = q @ K.T * SCALE
+                    z = q @ K.T * self.scale
                     # 128 products summed in fp32 in any order, then scaled: every step half a step off
-                    dz = 132 * U * SCALE * (q.abs() @ K.abs().T)
+                    dz = 132 * U * abs(self.scale) * (q.abs() @ K.abs().T)
                     if self.softcap:
                         z = self.softcap * torch.tanh(z / self.softcap)   # slope at most 1; tanh itself to 8 half steps
                         dz = dz + 8 * U * z.abs()
@@ -194,7 +195,7 @@ class DenseProblem:
         prefix = self.prefix
         if isinstance(prefix, (list, tuple)):
             prefix = torch.tensor(prefix, dtype=torch.int32, device=device)
-        return ops.ScoreRule(scale=SCALE, softcap=self.softcap, window=self.window, prefix=prefix,
+        return ops.ScoreRule(scale=self.scale, softcap=self.softcap, window=self.window, prefix=prefix,
                              slopes=None if self.slopes is None else self.slopes.to(device),
                              docs=None if self.docs is None else self.docs.to(device))
 

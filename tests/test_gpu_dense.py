@@ -79,6 +79,14 @@ def test_score_rules(dtype, kw):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("kw", [dict(), dict(softcap=5.0, slopes=True), dict(window=90, prefix=4)])
+@pytest.mark.parametrize("scale", [-0.11, 0.0])
+def test_scales_that_are_not_positive(dtype, kw, scale):
+    check(DenseProblem([700, 333, 2, 0], [1] * 4, dtype=dtype, seed=22, scale=scale, **kw), mass=True)
+
+
+@gpu
 def test_long_split_range_and_large_scores():
     check(DenseProblem([40000, 17], [1, 1], heads=1, groups=2, dtype=HF, seed=5, q_gain=6.0), mass=True)
 

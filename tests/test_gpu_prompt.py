@@ -99,6 +99,14 @@ def test_score_rules(dtype, kw):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("kw", [dict(), dict(softcap=5.0, slopes=True), dict(window=50, prefix=4, docs=3)])
+@pytest.mark.parametrize("scale", [-0.11, 0.0])
+def test_scales_that_are_not_positive(dtype, kw, scale):
+    check(PromptProblem([300, 133, 2, 0], [300, 60, 2, 0], dtype=dtype, heads=2, groups=2, seed=22, pad=2, scale=scale, **kw), mass=0)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("rows_max", [0, 5])
 def test_few_rows_on_a_long_cache_split_and_joined(dtype, rows_max):
@@ -253,6 +261,14 @@ def test_rows_enough_for_the_large_workgroups(dtype, kw):
     if "docs" in kw:
         p.docs = torch.randint(0, 3, p.docs.shape, generator=torch.Generator().manual_seed(5)).to(torch.int32)
     check(p, mass=3)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("kw", [dict(slopes=True), dict(scale=-0.11), dict(scale=0.0, window=300)])
+def test_biased_scores_and_other_scales_in_the_large_workgroups(dtype, kw):
+    check(PromptProblem([901, 700, 512, 900, 650, 640, 577, 830], [512, 500, 512, 550, 520, 515, 490, 500], heads=2, groups=16,
+                        dtype=dtype, seed=46, **kw), mass=3)
 
 
 @gpu
