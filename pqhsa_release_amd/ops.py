@@ -101,6 +101,8 @@ def kv_contiguous(keys: torch.Tensor, values: torch.Tensor) -> KvSource:
         raise ValueError(f"keys/values must be [B, H, S, {HEAD_DIM}]")
     if keys.stride() != values.stride() or keys.stride(-1) != 1 or keys.dtype != values.dtype:
         raise ValueError("keys and values must share dtype and strides, last dim contiguous")
+    if any(v < k for k, v in zip(keys.shape, values.shape)):
+        raise ValueError(f"values {tuple(values.shape)} do not cover the shape of the keys {tuple(keys.shape)}")
     v = KvView()
     v.k_base, v.v_base = keys.data_ptr(), values.data_ptr()
     v.dtype, v.paged = dtype_code(keys.dtype), 0

@@ -295,6 +295,15 @@ def test_refusals():
     refused("docs", rule=ops.ScoreRule(scale=SCALE, docs=torch.zeros(2, 63, dtype=torch.int32, device="cuda")))
 
 
+@gpu
+def test_values_for_fewer_sequences_or_tokens_than_the_keys_are_refused():
+    keys = torch.zeros(2, 2, 10, DIM, device="cuda")
+    for values in (keys[:1], keys[:, :1], keys[:, :, :5]):       # (of the same strides)
+        assert values.stride() == keys.stride()
+        with pytest.raises(ValueError, match="shape"):
+            ops.kv_contiguous(keys, values)
+
+
 def test_rule_refusals_without_a_gpu():
     for kw in (dict(scale=math.nan), dict(scale=1.0, softcap=-1.0), dict(scale=1.0, softcap=math.inf), dict(scale=1.0, window=-1),
                dict(scale=1.0, prefix=-2), dict(scale=1.0, prefix=torch.zeros(2)), dict(scale=1.0, slopes=torch.zeros(2)),
