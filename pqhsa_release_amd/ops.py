@@ -753,6 +753,7 @@ def hybrid_attend_paged(q, out, kv: KvSource, index: DeviceIndex, groups: int, s
 
 # --------------------------------------------------------------------------- dense attention
 MAX_GROUPS = 16
+_INT32_MAX = 2**31 - 1      # (ctypes cuts longer numbers off without a word)
 
 
 class ScoreRule:
@@ -766,16 +767,16 @@ class ScoreRule:
                  slopes: torch.Tensor | None = None, docs: torch.Tensor | None = None) -> None:
         s = _lib.Score()
         s.scale, s.softcap, s.window = float(scale), float(softcap), int(window)
-        if not math.isfinite(s.scale) or not math.isfinite(s.softcap) or s.softcap < 0 or s.window < 0:
-            raise ValueError("scale must be finite, softcap finite and not negative, window not negative")
+        if not math.isfinite(s.scale) or not math.isfinite(s.softcap) or s.softcap < 0 or not 0 <= int(window) <= _INT32_MAX:
+            raise ValueError("scale must be finite, softcap finite and not negative, window in [0, 2^31)")
         if isinstance(prefix, torch.Tensor):
             if prefix.dtype != torch.int32 or prefix.ndim != 1 or not prefix.is_contiguous():
                 raise ValueError("prefix must be an int or a contiguous int32 [B] tensor")
             s.prefixes = prefix.data_ptr()
         elif prefix is not None:
             s.prefix = int(prefix)
-            if s.prefix < 0:
-                raise ValueError("prefix must not be negative")
+            if not 0 <= int(prefix) <= _INT32_MAX:
+                raise ValueError("prefix must lie in [0, 2^31)")
         if slopes is not None:
             if slopes.dtype != torch.float32 or slopes.ndim != 1 or not slopes.is_contiguous():
                 raise ValueError("slopes must be a contiguous float32 [H*G] tensor")
@@ -900,8 +901,8 @@ def _mass_struct(mass, mass_in, decay: float, rows: int, batch: int, heads: int,
             raise ValueError("mass_in must have the shape of mass")
         if 0 < abs(mass_in.data_ptr() - mass.data_ptr()) < mass.numel() * 4:
             raise ValueError("mass_in must be mass itself or lie apart from it")
-    if not math.isfinite(float(decay)) or rows < 0:
-        raise ValueError("decay must be finite, mass_rows not negative")
+    if not math.isfinite(float(decay)) or not 0 <= rows <= _INT32_MAX:
+        raise ValueError("decay must be finite, mass_rows in [0, 2^31)")
     m = _lib.Mass()
     m.in_, m.out, m.stride = _ptr(mass_in), mass.data_ptr(), mass.shape[2]
     m.decay, m.rows = float(decay), int(rows)
@@ -909,8 +910,8 @@ def _mass_struct(mass, mass_in, decay: float, rows: int, batch: int, heads: int,
 
 
 def _check_bound(kv: KvSource, n_max: int) -> None:
-    if n_max < 0 or n_max > kv.capacity:
-        raise ValueError(f"n_max {n_max} outside [0, {kv.capacity}], the tokens the cache can hold per sequence")
+    if n_max < 0 or n_max > min(kv.capacity, _INT32_MAX):
+        raise ValueError(f"n_max {n_max} outside [0, {min(kv.capacity, _INT32_MAX)}], the tokens the cache can hold per sequence")
 
 
 class DenseAttendCall:
@@ -1021,8 +1022,8 @@ def evict(kv: KvSource, dst: KvSource, mass: torch.Tensor, seq_lens: torch.Tenso
     device = _one_device(mass, (kv, dst), seq_lens, mass_out)
     if dst.batch != b or dst.kv_heads != h or dst.dtype != kv.dtype:
         raise ValueError("dst must have the batch, KV heads and dtype of kv")
-    if sink < 0 or recent < 0 or keep < 1 or sink + recent > keep:
-        raise ValueError(f"keep {keep} must be positive and hold sink {sink} + recent {recent}")
+    if sink < 0 or recent < 0 or not 1 <= keep <= _INT32_MAX or sink + recent > keep:
+        raise ValueError(f"keep {keep} must be positive, below 2^31 and hold sink {sink} + recent {recent}")
     _check_bound(kv, n_max)
     left = min(keep, n_max)
     if dst.capacity < left:

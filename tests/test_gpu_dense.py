@@ -312,6 +312,28 @@ def test_rule_refusals_without_a_gpu():
             ops.ScoreRule(**kw)
 
 
+def test_numbers_of_more_than_32_bits_are_refused():
+    for kw in (dict(window=2**32 + 5), dict(window=2**31), dict(prefix=2**32 + 3), dict(prefix=2**31)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            ops.ScoreRule(scale=1.0, **kw)
+    assert ops.ScoreRule(scale=1.0, window=2**31 - 1, prefix=2**31 - 1).struct.window == 2**31 - 1
+    mass = torch.zeros(1, 1, 8)
+    with pytest.raises(ValueError, match="mass_rows"):
+        ops._mass_struct(mass, None, 1.0, 2**32 + 1, 1, 1, 8)
+    for n_max in (2**31, 2**32 + 8):
+        with pytest.raises(ValueError, match="n_max"):
+            ops._check_bound(ops.KvSource(None, (), torch.float32, 1, 1, 2**33), n_max)
+
+
+@gpu
+def test_kept_keys_of_more_than_32_bits_are_refused():
+    kv = ops.kv_contiguous(*torch.zeros(2, 1, 1, 8, DIM, device="cuda"))
+    dst = ops.kv_contiguous(*torch.zeros(2, 1, 1, 8, DIM, device="cuda"))
+    with pytest.raises(ValueError, match="keep"):
+        ops.evict(kv, dst, torch.zeros(1, 1, 8, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda"), keep=2**32 + 4,
+                  sink=1, recent=1, n_max=8)
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: a call that were not refused must find no GPU")
 def test_c_entry_refuses_bad_arguments_before_any_gpu_work():
     import ctypes
