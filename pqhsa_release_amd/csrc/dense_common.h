@@ -34,29 +34,36 @@ constexpr float kMaxSlack = 8.0f;
 // kernel's) below it: keys far below the largest one, which only count together (those behind an attention
 // sink, say), then have the same bits.  It stays within 2^40 of the row's maximum: what is rounded away below that is
 // under 2^31 keys * 2^-78 * 2^16, less than fp16 outputs resolve.  Sums hold 2^15 * 2^40 * 2^16 * 2^31 keys.
-// This base is an integer, its moves exact.
+// A new maximum becomes the base itself, up to 2^-15 (the weight of a key that stands out is then a power of two,
+// and not rounded); all other moves are by whole numbers, and exact, as multiples of 2^-14 below 2^10 are.
 constexpr float kHalfSlack = 2.0f, kHalfShift = 13.0f, kHalfFall = 40.0f;
 template <int DT>
 struct WeightBase {
     static constexpr bool kHalf = DT == PQHSA_F16;
     static constexpr float kSlack = kHalf ? kHalfSlack : kMaxSlack;
     float m = -INFINITY;                                 // the base; -inf: no visible key so far
-    float most = -INFINITY;                              // fp16: the row's maximum so far, rounded up
+    float most = -INFINITY;                              // fp16: the row's maximum so far
     __device__ inline bool raises(float top) const { return top > m + kSlack; }
     __device__ inline bool falls(float top, float drop) const { return kHalf && top < m - drop; }
     // moves to a tile's maximum `top` of the row; returns what sums so far are multiplied by
     __device__ inline float move(float top, float drop) {
-        float to = fmaxf(m, top), f;
         if constexpr (kHalf) {
-            to = ceilf(to);
-            most = fmaxf(most, to);
-            if (falls(top, drop) && top > -INFINITY && m < INFINITY) to = fmaxf(ceilf(top), most - kHalfFall);
-            f = m == to ? 1.0f : __builtin_ldexpf(1.0f, (int)fmaxf(m - to, -200.0f));
+            if (top > most) {
+                const float to = (top + 768.0f) - 768.0f, f = exp2_fast(m - to);   // (the sum drops what is below 2^-14)
+                m = to;
+                most = top;
+                return f;
+            }
+            float by = 0.0f;                             // upwards
+            if (top > m) by = ceilf(top - m);
+            else if (falls(top, drop) && top > -INFINITY && m < INFINITY) by = -fminf(floorf(m - top), floorf(m - most + kHalfFall));
+            m += by;
+            return __builtin_ldexpf(1.0f, -(int)by);
         } else {
-            f = m == to ? 1.0f : exp2_fast(m - to);
+            const float to = fmaxf(m, top), f = m == to ? 1.0f : exp2_fast(m - to);
+            m = to;
+            return f;
         }
-        m = to;
-        return f;
     }
     // what exponents are taken relative to
     __device__ inline float origin() const { return m == -INFINITY ? 0.0f : kHalf ? m - kHalfShift : m; }

@@ -239,6 +239,18 @@ def test_an_infinite_value_of_a_key_with_next_to_no_weight(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("at", [0, 37, 700])
+def test_a_key_that_stands_out_gives_its_value_unrounded(dtype, at):
+    """All other weights together are under 1500 * exp(-30 + 5) = 2e-8: what is off beyond that (and beyond 2^-15, where
+    fp16's base is cut) is a rounding of the one weight, which is avoidable."""
+    p = DenseProblem([1500, 801], [1, 1], heads=2, groups=2, dtype=dtype, seed=71).set_levels([30.37 if j == at else 0.0 for j in range(1500)], spread=1.0)
+    out, _, _, _ = run(p)
+    want = p.V[:, :, at].repeat_interleave(2, 1)
+    assert torch.equal(out.cpu(), want)
+
+
+@gpu
 def test_rows_beyond_32_bit_offsets():
     p = DenseProblem([300, 77], [1, 1], heads=8, groups=4, layout="5d", block=16, seed=17)
     near, q, sl, rule = p.source(), p.q.cuda(), p.seq_lens(), p.rule()

@@ -226,6 +226,18 @@ def test_infinite_values_in_the_large_workgroups(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("at", [0, 37, 700])
+def test_a_key_that_stands_out_gives_its_value_unrounded(dtype, at):
+    """All other weights together are under 1500 * exp(-30 + 5) = 2e-8: what is off beyond that (and beyond 2^-15, where
+    fp16's base is cut) is a rounding of the one weight, which is avoidable."""
+    p = PromptProblem([1500, 801], [700, 4], heads=2, groups=2, dtype=dtype, seed=71).set_levels([30.37 if j == at else 0.0 for j in range(1500)], spread=1.0)
+    out, _, _, _ = run(p)
+    want = p.V[:, :, at].repeat_interleave(2, 1)
+    assert torch.equal(out.cpu(), torch.cat([want[:1].expand(700, -1, -1), want[1:].expand(4, -1, -1)]))
+
+
+@gpu
 def test_block_table_entries_outside_the_cache_mask_their_keys():
     kw = dict(heads=2, groups=2, block=16, poison=False, seed=9)
     p, q = PromptProblem([160], [160], **kw), PromptProblem([160], [160], **kw)
