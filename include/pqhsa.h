@@ -455,8 +455,8 @@ int pqhsa_hybrid_attend_paged(const void *q, int32_t q_dtype, void *out,
  * and the row sees key j when j lies in the sequence, docs[b, i] == docs[b, j], and either
  * j <= i and (window == 0 or i - j < window), or j < the sequence's prefix.  (A prefix with a window
  * keeps the first tokens in sight, a prefix as long as the sequence lifts the causal order.)  Masked
- * keys may hold anything, infinities and NaN included.  A row that sees nothing gives 0, its
- * log-sum-exp -inf.  Positions are slots of the cache: after an eviction distances count the keys
+ * keys may hold anything, infinities and NaN included; an infinite value that a row sees makes the row's
+ * element infinite, however small its weight.  A row that sees nothing gives 0, its log-sum-exp -inf.  Positions are slots of the cache: after an eviction distances count the keys
  * that are left.
  */
 typedef struct pqhsa_score {
@@ -506,7 +506,8 @@ int pqhsa_dense_attend_paged(const void *q, int32_t q_dtype, int64_t q_stride_ro
  * sequence (more rows than tokens) sees nothing.  lse f32 [T, H * G], mass: may be NULL.  rows_hint:
  * the largest number of rows of a sequence, 0 = unknown (sizes the launch, results do not depend on
  * it beyond summation order).  n_max, blocks, workspace: as above; `with_mass` is 0 when mass is NULL.
- * B * H <= 65535, T * H * G < 2^31; with docs, n_max up to about a million (a bit per key tile in LDS).
+ * B * H <= 65535, T * H * G < 2^31; with docs, n_max up to 3 million in fp32 and 6 million in the 2-byte types (two bits
+ * per key tile in LDS).
  */
 size_t pqhsa_prompt_attend_workspace_bytes(int64_t T, int32_t B, int32_t H, int32_t G, int32_t n_max,
                                            int32_t rows_hint, int32_t dtype, int32_t with_mass);

@@ -20,9 +20,10 @@
 // rounded remainder), because a second product costs nothing here: 2^-17 of a weight is rounded away at most in
 // bf16, 2^-22 in fp16 (there by a base near the step's own scores, and a remainder of its own scale).
 //
-// Measured (bf16, 16-token pages): 4 x 131 072 tokens of 8 KV heads 392 us, 5.5 TB/s; 1 x 32 768 30 us, 26 of them
-// the attention at 5.1 TB/s and 4 the join; 16 x 700 12 us, which are two launches and the chain
-// length -> block -> row -> partial -> output, not bytes.
+// Measured (bf16, 16-token pages): 4 x 131 072 tokens of 8 KV heads 392 us, 5.5 TB/s; 1 x 32 768 34 us, 4 of them
+// the join (30 us called again and again on one cache of 134 MB, part of which then stays in the last-level
+// cache); 16 x 700 12 to 15 us, which are two launches and the chain length -> block -> row -> partial -> output, not
+// bytes.  The launch is sized by the bound of the lengths: 1 x 8 192 takes 15 us under its own, 33 under 131 072.
 #include "dense_common.h"
 
 namespace pqhsa {
@@ -572,8 +573,8 @@ DensePlan plan_dense(int B, int H, int G, int n_max, const pqhsa_score *score, b
     const int64_t streams = (int64_t)B * H;
     const int64_t keys = visible_bound(score, n_max) > 0 ? visible_bound(score, n_max) : 1;
     // The chip holds 512 workgroups at once.  One sequence's chunks are equally long, so it is cut into one
-    // such round (1 x 32768: 30.8 us, 33.7 in three rounds); several are as long as the longest at most, and
-    // three rounds even that out (16 of 16384 to 65536 keys: 360 us, 381 in two).
+    // such round (1 x 32768, one resident cache: 30.8 us, 33.7 in three rounds); several are as long as the longest at
+    // most, and three rounds even that out (16 of 16384 to 65536 keys: 360 us, 381 in two).
     const int64_t want = B == 1 ? 512 : 1536;
     int64_t chunk = (streams * keys + want - 1) / want;
     // No join where it costs more than walking on: two steps a wave (8 heads of 256 keys 8.9 us, 10.2 joined), and
